@@ -367,6 +367,63 @@ int kfh_single_track_forward(const void* z, void* s, const uint8_t* token_mask, 
                              size_t workspace_bytes, int B, int N, int Cz, int Cs, int H, int expansion,
                              float eps, int io_dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Training operators: the forms of layer norm, the gated feed-forward block and dropout that a
+ * training step of the transition and of the pair track's residual adds needs.  Nothing but the
+ * operators' inputs (and two fp32 statistics per row of the layer norm) is kept between a forward
+ * and its backward call.  Sums over rows are taken in a fixed order: the same call gives the same
+ * bits.
+ * ------------------------------------------------------------------------------------- */
+
+/* Layer norm over the last dimension (model/primitives/normalization.py:61-91):
+ *   y[r,c] = (x[r,c] - mean[r]) * rstd[r] * weight[c] + bias[c],  rstd = (var + eps)^-1/2
+ * x, y: [rows, C] of io_dtype, any C from 1 to 65536; weight, bias: fp32 [C] or NULL (1 / 0);
+ * mean, rstd: fp32 [rows], both or neither NULL (what the backward call takes).  Statistics are
+ * fp32.  `y` may be `x`. */
+int kfh_layer_norm_forward(const void* x, const float* weight, const float* bias, void* y, float* mean,
+                           float* rstd, long long rows, int C, float eps, int io_dtype, void* stream);
+
+/* dx = rstd * (a - mean_c(a) - xh * mean_c(a * xh)) with xh = (x - mean) * rstd, a = dy * weight;
+ * dweight[c] = sum_r dy * xh, dbias[c] = sum_r dy (fp32 [C]).  dx, dweight and dbias may each be
+ * NULL; without the last two no workspace is needed.  `dx` may be `dy`.  rows = 0 gives zero
+ * dweight and dbias. */
+size_t kfh_layer_norm_backward_workspace_bytes(long long rows, int C);
+int kfh_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd,
+                            const float* weight, void* dx, float* dweight, float* dbias, void* workspace,
+                            size_t workspace_bytes, long long rows, int C, int io_dtype, void* stream);
+
+/* Gated feed-forward block (model/primitives/activation.py:20-29 with the output projection of
+ * model/layers/folding/transition.py:48-68):
+ *   [u; v] = x w_in^T,  y = (silu(u) * v) w_out^T;  x, y: [rows, C], w_in: [2F, C], w_out: [C, F],
+ * all row-major of io_dtype, C and F multiples of 8, pointers 16-byte aligned.  KFH_BF16: bf16
+ * matrix products with fp32 accumulation, hidden values rounded to bf16 between the products;
+ * KFH_F32: products carried to fp32 accuracy (as KFH_ARITH_F32), hidden values kept in fp32. */
+size_t kfh_gated_ffn_workspace_bytes(long long rows, int C, int F, int backward, int io_dtype);
+int kfh_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, void* y, void* workspace,
+                          size_t workspace_bytes, long long rows, int C, int F, int io_dtype, void* stream);
+
+/* Gradients for dy [rows, C]: dx [rows, C] (io_dtype), dw_in [2F, C] and dw_out [C, F] (dw_dtype);
+ * each may be NULL.  u and v are computed again from x.  `dx` may be `dy`.  rows = 0 gives zero
+ * weight gradients. */
+int kfh_gated_ffn_backward(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx,
+                           void* dw_in, void* dw_out, int dw_dtype, void* workspace, size_t workspace_bytes,
+                           long long rows, int C, int F, int io_dtype, void* stream);
+
+/* Dropout (model/primitives/dropout.py:65) with a mask that is computed where it is used and never
+ * stored:   y = (residual ? residual : 0) + (keep ? x * scale : 0)
+ * x, residual, y: [outer, shared, inner] of io_dtype, any sizes; one mask value covers the `shared`
+ * dimension (1: a value per element; the row length or the number of rows: row- / column-wise
+ * dropout of the pair track).  t = round(p * 2^16), keep where the element's 16 random bits are
+ * >= t, scale = 2^16 / (2^16 - t); p = 1 leaves the residual.  Element i of [outer, inner] takes
+ * half-word i % 8 of Philox4x32-10 at counter (i / 8, offset) under the key `seed`, or under the
+ * 64-bit value `seed_dev` points at in device memory (read when the kernel runs, so that a captured
+ * call can be replayed with new masks); pass seed_dev = NULL for an immediate seed.  The gradient
+ * with respect to x is the same call on dy without residual; dropped elements are 0 whatever x
+ * holds there.  `y` may be `x` or `residual`. */
+int kfh_dropout(const void* x, const void* residual, void* y, long long outer, long long shared,
+                long long inner, double p, const unsigned long long* seed_dev, unsigned long long seed,
+                unsigned long long offset, int io_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ The library is loaded on first use.  There is no fallback: if it has not been bu
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_size_t, c_ulonglong, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libkfold_hip.so"
@@ -74,6 +74,14 @@ SIGNATURES: dict[str, tuple] = {
     "kfh_parcae_packed_bytes": (c_size_t, [c_int]),
     "kfh_parcae_pack": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, _P, _P]),
     "kfh_parcae_step": (c_int, [_P, _P, _P, _P, _P, c_longlong, c_int, c_float, c_int, _P]),
+    "kfh_layer_norm_forward": (c_int, [_P, _P, _P, _P, _P, _P, c_longlong, c_int, c_float, c_int, _P]),
+    "kfh_layer_norm_backward_workspace_bytes": (c_size_t, [c_longlong, c_int]),
+    "kfh_layer_norm_backward": (c_int, [_P] * 9 + [c_size_t, c_longlong, c_int, c_int, _P]),
+    "kfh_gated_ffn_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int, c_int, c_int]),
+    "kfh_gated_ffn_forward": (c_int, [_P] * 5 + [c_size_t, c_longlong, c_int, c_int, c_int, _P]),
+    "kfh_gated_ffn_backward": (c_int, [_P] * 7 + [c_int, _P, c_size_t, c_longlong, c_int, c_int, c_int, _P]),
+    "kfh_dropout": (c_int, [_P, _P, _P, c_longlong, c_longlong, c_longlong, c_double, _P, c_ulonglong, c_ulonglong,
+                            c_int, _P]),
 }
 
 _lib = None

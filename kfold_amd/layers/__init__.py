@@ -8,4 +8,4 @@ from .attention_pair_bias import (  # noqa: F401
     hip_attention_pair_bias,
     prepare_pair_bias,
 )
-from .transition import SwiGLU, Transition, hip_transition  # noqa: F401
+from .transition import SwiGLU, Transition, hip_transition, hip_transition_train  # noqa: F401

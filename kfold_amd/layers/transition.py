@@ -3,6 +3,10 @@
 Mirror of the reference's ``Transition`` (src/kfold/model/layers/folding/transition.py:20-68)
 and ``SwiGLU`` (model/primitives/activation.py:20-29): same constructor and parameter names
 (``layernorm``, ``swiglu.linear``, ``linear_out``).
+
+Without gradients ``Transition`` is one fused call on packed weights (``hip_transition``); with
+gradients enabled it is the layer norm and the gated feed-forward block of ``kfold_amd.functional``
+(``hip_transition_train``), which differentiate with respect to x and every parameter.
 """
 
 from __future__ import annotations
@@ -10,7 +14,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from .. import ops
+from .. import functional, ops
 from ..primitives._common import cache_key, cached_blob, check_inference
 from ..primitives.layers import LayerNorm, LinearNoBias
 
@@ -36,6 +40,21 @@ def hip_transition(module: nn.Module, x: torch.Tensor, residual: torch.Tensor | 
     return res.to(x.dtype)
 
 
+def _autocast_dtype(x: torch.Tensor) -> torch.dtype:
+    if torch.is_autocast_enabled(x.device.type):
+        return torch.get_autocast_dtype(x.device.type)
+    return x.dtype
+
+
+@torch.compiler.disable
+def hip_transition_train(module: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``Transition(x)`` with gradients; x [..., C].  bf16 tensors (and fp32 ones under bf16 autocast)
+    run bf16 matrix products, fp32 tensors products of fp32 accuracy."""
+    ln = module.layernorm
+    xn = functional.layer_norm(x, ln.weight, ln.bias, ln.eps).to(_autocast_dtype(x))
+    return functional.gated_ffn(xn, module.swiglu.linear.weight, module.linear_out.weight).to(x.dtype)
+
+
 class SwiGLU(nn.Module):
     def __init__(self, channel_in: int, channel_out: int):
         super().__init__()
@@ -51,4 +70,4 @@ class Transition(nn.Module):
         self.linear_out = LinearNoBias(self.model_dim, channel, init="final")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return hip_transition(self, x)
+        return hip_transition_train(self, x) if torch.is_grad_enabled() else hip_transition(self, x)

@@ -297,8 +297,8 @@ class ParcaeTrunk(ParcaeStep):
     Sub-modules and parameters carry the names they have on the reference's ``KFold`` (``lm_stack``,
     ``main_stack``, ``layernorm_z``, ``parcae_log_a``, ``parcae_log_delta``, ``parcae_b_cont``), so
     ``load_reference_weights`` fills them from a KFold state dict.  The reference draws a fresh
-    dropout mask on ``z_lm`` every recycle (:525); pass the already dropped-out tensor (or a
-    callable returning it) as ``z_lm``."""
+    dropout mask on ``z_lm`` every recycle (:525): pass ``lm_dropout`` and ``lm_seed``, or the already
+    dropped-out tensor (or a callable returning it) as ``z_lm``."""
 
     def __init__(self, channel_z: int = 256, lm_blocks: int = 4, main_blocks: int = 48,
                  decay_init: float = 0.4472135954999579, kernel_backend: str = "hip"):
@@ -307,12 +307,15 @@ class ParcaeTrunk(ParcaeStep):
         self.main_stack = TrianglularStack(channel_z, main_blocks, kernel_backend=kernel_backend)
 
     def forward(self, z: torch.Tensor, z_inputs: torch.Tensor, z_lm, pair_mask: torch.Tensor,
-                num_recycles: int = 0) -> torch.Tensor:
+                num_recycles: int = 0, lm_dropout: float = 0.0, lm_seed: int = 0) -> torch.Tensor:
         """z [B, N, N, C] (the pair state, updated in place), z_inputs [B, N, N, C], z_lm a tensor
-        or a callable giving this recycle's (dropped-out) LM pair embedding."""
-        for _ in range(num_recycles + 1):
+        or a callable giving this recycle's LM pair embedding.  With ``lm_dropout`` its values are
+        dropped with that probability, recycle r by the mask of (``lm_seed``, r)."""
+        for r in range(num_recycles + 1):
             lm_in = z_lm() if callable(z_lm) else z_lm
-            lm = self.lm_stack(lm_in.clone(), pair_mask)          # the stack works in place
+            # the stack works in place: on a copy, which the dropout writes if there is one
+            lm_in = ops.dropout_forward(lm_in, lm_dropout, lm_seed, r) if lm_dropout else lm_in.clone()
+            lm = self.lm_stack(lm_in, pair_mask)
             ParcaeStep.forward(self, z, lm, inplace=True, u_add=z_inputs.contiguous())
             z = self.main_stack(z, pair_mask)
         return z

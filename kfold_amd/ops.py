@@ -126,7 +126,8 @@ def workspace_bytes(op: str, **shape) -> int:
     """Bytes of scratch memory a forward call needs (0: shape not supported): ``trimul`` (N, C),
     ``triattn`` (N, C, heads) — both also with ``B``: the size that takes a batch through the kernels at
     once —, ``transition`` (rows, C, expansion), ``apb`` (S, L, C, heads,
-    cond_channels, arith), ``cross_apb`` (W, Lq, Lk, C, heads, cond_channels, arith).  Needs no GPU."""
+    cond_channels, arith), ``cross_apb`` (W, Lq, Lk, C, heads, cond_channels, arith),
+    ``layer_norm_backward`` (rows, C), ``gated_ffn`` (rows, C, F, backward, dtype).  Needs no GPU."""
     L = _lib.lib()
     g = shape.__getitem__
     if op == "trimul":
@@ -145,6 +146,11 @@ def workspace_bytes(op: str, **shape) -> int:
     if op == "cross_apb":
         return L.kfh_cross_apb_workspace_bytes(g("W"), g("Lq"), g("Lk"), g("C"), g("heads"),
                                                shape.get("cond_channels", 0), shape.get("arith", KFH_ARITH_BF16))
+    if op == "layer_norm_backward":
+        return L.kfh_layer_norm_backward_workspace_bytes(g("rows"), g("C"))
+    if op == "gated_ffn":
+        return L.kfh_gated_ffn_workspace_bytes(g("rows"), g("C"), g("F"), 1 if shape.get("backward") else 0,
+                                               _IO_DTYPES[shape.get("dtype", torch.bfloat16)])
     raise ValueError(f"unknown op {op!r}")
 
 
@@ -562,3 +568,214 @@ def cross_apb_forward(a_q: torch.Tensor, a_k: torch.Tensor, s_q, s_k, pair_bias:
                                       cond_channels, 1 if apply_norm else 0, float(eps), _io_dtype(aq), arith,
                                       _stream(dev)))
     return out
+
+
+# ---------------------------------------------------------------------------------------
+# training operators: layer norm, gated feed-forward block, dropout
+# ---------------------------------------------------------------------------------------
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and at a 16-byte boundary (a view into a larger tensor may start anywhere)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _result(out: torch.Tensor | None, like: torch.Tensor, name: str, aligned: bool = False) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(like)
+    if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with the shape and dtype of {tuple(like.shape)} {like.dtype}")
+    if aligned and out.data_ptr() % 16:
+        raise ValueError(f"{name} must be aligned to 16 bytes")
+    return out
+
+
+def _affine_f32(w: torch.Tensor | None, C: int, name: str) -> torch.Tensor | None:
+    if w is None:
+        return None
+    if w.shape != (C,):
+        raise ValueError(f"layer norm: {name} has shape {tuple(w.shape)}, the rows have {C} channels")
+    return w.detach().to(dtype=torch.float32).contiguous()
+
+
+def _rows(x: torch.Tensor) -> tuple[int, int]:
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"rows of at least one channel are needed, got shape {tuple(x.shape)}")
+    return x.numel() // x.shape[-1], x.shape[-1]
+
+
+def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                       eps: float = 1e-5, stats: bool = False, out: torch.Tensor | None = None):
+    """Layer norm over the last dim of x (any width); weight and bias [C] or None.  With ``stats``
+    returns ``(y, mean, rstd)``, the fp32 row statistics ``layer_norm_backward`` takes, else y."""
+    dev = _require_cuda(x, weight, bias, out)
+    io = _io_dtype(x)
+    rows, C = _rows(x)
+    xc = x.contiguous()
+    y = _result(out, xc, "out")
+    w, b = _affine_f32(weight, C, "weight"), _affine_f32(bias, C, "bias")
+    mean = rstd = None
+    if stats:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    if rows:
+        with torch.cuda.device(dev):
+            check(_lib.lib().kfh_layer_norm_forward(xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(mean),
+                                                    _ptr(rstd), rows, C, float(eps), io, _stream(dev)))
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                        weight: torch.Tensor | None = None, need_dx: bool = True, need_dparams: bool = True,
+                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """``(dx, dweight, dbias)`` of ``layer_norm_forward``: dx like x, dweight and dbias fp32 [C] (sums
+    over all rows, in a fixed order), None for what is not needed.  ``out`` (for dx) may be dy;
+    ``workspace`` as in ``trimul_forward`` (``workspace_bytes("layer_norm_backward", rows=, C=)``)."""
+    dev = _require_cuda(dy, x, mean, rstd, weight, out)
+    io = _io_dtype(x)
+    rows, C = _rows(x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy must have the shape and dtype of x, got {tuple(dy.shape)} {dy.dtype}")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.numel() != rows or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 with one value per row")
+    xc, dyc = x.contiguous(), dy.contiguous()
+    w = _affine_f32(weight, C, "weight")
+    dx = _result(out, xc, "out") if need_dx else None
+    dw = db = ws = None
+    ws_bytes = 0
+    L = _lib.lib()
+    if need_dparams:
+        dw = torch.empty((C,), dtype=torch.float32, device=dev)
+        db = torch.empty((C,), dtype=torch.float32, device=dev)
+        ws_bytes = L.kfh_layer_norm_backward_workspace_bytes(rows, C)
+        ws = _workspace(workspace, ws_bytes, dev)
+    if dx is not None or dw is not None:
+        with torch.cuda.device(dev):
+            check(L.kfh_layer_norm_backward(dyc.data_ptr(), xc.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(w),
+                                            _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, rows, C, io,
+                                            _stream(dev)))
+    return dx, dw, db
+
+
+def _ffn_shapes(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> tuple[int, int, int]:
+    rows, C = _rows(x)
+    if w_in.dim() != 2 or w_out.dim() != 2 or w_in.shape[1] != C or w_in.shape[0] % 2 \
+            or w_out.shape != (C, w_in.shape[0] // 2):
+        raise ValueError(f"gated feed-forward: rows of {C} channels need w_in [2F, {C}] and w_out [{C}, F], got "
+                         f"{tuple(w_in.shape)} and {tuple(w_out.shape)}")
+    if w_in.dtype != x.dtype or w_out.dtype != x.dtype:
+        raise TypeError(f"gated feed-forward: x, w_in and w_out must have one dtype, got {x.dtype}, {w_in.dtype}, "
+                        f"{w_out.dtype}")
+    F = w_out.shape[1]
+    if C % 8 or F % 8 or F == 0:
+        raise NotImplementedError(f"hip gated feed-forward: C={C}, F={F} unsupported (multiples of 8)")
+    return rows, C, F
+
+
+def gated_ffn_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``(silu(u) * v) w_out^T`` with ``u, v = chunk(x w_in^T, 2)`` over the last dim of x; w_in [2F, C],
+    w_out [C, F], C and F multiples of 8, one dtype: bf16, or fp32 with products of fp32 accuracy.
+    ``workspace`` as in ``trimul_forward`` (``workspace_bytes("gated_ffn", rows=, C=, F=, backward=,
+    dtype=)``)."""
+    dev = _require_cuda(x, w_in, w_out, out)
+    io = _io_dtype(x)
+    rows, C, F = _ffn_shapes(x, w_in, w_out)
+    xc = _aligned(x)
+    y = _result(out, xc, "out", aligned=True)
+    if rows == 0:
+        return y
+    wi, wo = _aligned(w_in), _aligned(w_out)
+    L = _lib.lib()
+    ws_bytes = L.kfh_gated_ffn_workspace_bytes(rows, C, F, 0, io)
+    ws = _workspace(workspace, ws_bytes, dev) if ws_bytes else None
+    with torch.cuda.device(dev):
+        check(L.kfh_gated_ffn_forward(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr(), _ptr(ws), ws_bytes,
+                                      rows, C, F, io, _stream(dev)))
+    return y
+
+
+def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
+                       need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype | None = None,
+                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """``(dx, dw_in, dw_out)`` of ``gated_ffn_forward`` for the gradient dy of its result (the hidden
+    values are computed again from x); the weight gradients in ``dw_dtype`` (default: the weights'),
+    None for what is not needed.  ``out`` (for dx) may be dy."""
+    dev = _require_cuda(dy, x, w_in, w_out, out)
+    io = _io_dtype(x)
+    rows, C, F = _ffn_shapes(x, w_in, w_out)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy must have the shape and dtype of x, got {tuple(dy.shape)} {dy.dtype}")
+    dw_dtype = w_in.dtype if dw_dtype is None else dw_dtype
+    if dw_dtype not in _IO_DTYPES:
+        raise TypeError(f"hip backend supports bfloat16 and float32 tensors, got dw_dtype={dw_dtype}")
+    xc, dyc, wi, wo = _aligned(x), _aligned(dy), _aligned(w_in), _aligned(w_out)
+    dx = _result(out, xc, "out", aligned=True) if need_dx else None
+    dwi = dwo = None
+    if need_dw:
+        dwi = torch.empty(tuple(w_in.shape), dtype=dw_dtype, device=dev)
+        dwo = torch.empty(tuple(w_out.shape), dtype=dw_dtype, device=dev)
+    if not (need_dx or need_dw):
+        return None, None, None
+    L = _lib.lib()
+    ws_bytes = L.kfh_gated_ffn_workspace_bytes(rows, C, F, 1, io)
+    ws = _workspace(workspace, ws_bytes, dev) if rows else None
+    with torch.cuda.device(dev):
+        check(L.kfh_gated_ffn_backward(dyc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), _ptr(dx), _ptr(dwi),
+                                       _ptr(dwo), _IO_DTYPES[dw_dtype], _ptr(ws), ws_bytes, rows, C, F, io,
+                                       _stream(dev)))
+    return dx, dwi, dwo
+
+
+def _drop(x, residual, p, seed, offset, shared_dim, out):
+    dev = _require_cuda(x, residual, out, seed if isinstance(seed, torch.Tensor) else None)
+    io = _io_dtype(x)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p={p} is no probability")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have the shape and dtype of x")
+    outer, shared, inner = 1, 1, x.numel()
+    if shared_dim is not None:
+        if not -x.dim() <= shared_dim < x.dim():
+            raise ValueError(f"dropout: no dimension {shared_dim} in a tensor of {x.dim()}")
+        d = shared_dim % x.dim()
+        outer = inner = 1
+        shared = x.shape[d]
+        for n in x.shape[:d]:
+            outer *= n
+        for n in x.shape[d + 1:]:
+            inner *= n
+    seed_ptr, seed_val = None, 0
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError("dropout: a seed in device memory is one int64")
+        seed_ptr = seed.data_ptr()
+    else:
+        seed_val = int(seed) & 0xFFFFFFFFFFFFFFFF
+    xc = x.contiguous()
+    rc = None if residual is None else residual.contiguous()
+    y = _result(out, xc, "out")
+    if x.numel() == 0:
+        return y
+    with torch.cuda.device(dev):
+        check(_lib.lib().kfh_dropout(xc.data_ptr(), _ptr(rc), y.data_ptr(), outer, shared, inner, float(p), seed_ptr,
+                                     seed_val, int(offset) & 0xFFFFFFFFFFFFFFFF, io, _stream(dev)))
+    return y
+
+
+def dropout_forward(x: torch.Tensor, p: float, seed, offset: int = 0, shared_dim: int | None = None,
+                    residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``(residual or 0) + dropout(x)``: each value is dropped with probability p (taken to the nearest
+    multiple of 2^-16) and the kept ones are scaled by 1 / (1 - p).  The mask is a function of
+    (seed, offset, position) alone and is never stored; with ``shared_dim`` one mask value covers that
+    dimension (row- or column-wise dropout of a pair tensor).  ``seed`` is an int, or one int64 in
+    device memory, read when the kernel runs (a captured call then draws a new mask per replay);
+    two calls draw independent masks if they differ in seed or offset.  ``out`` may be x or residual."""
+    return _drop(x, residual, p, seed, offset, shared_dim, out)
+
+
+def dropout_backward(dy: torch.Tensor, p: float, seed, offset: int = 0, shared_dim: int | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of ``dropout_forward`` with respect to x (the residual's is dy itself): dy through the
+    same mask, computed again from (seed, offset)."""
+    return _drop(dy, None, p, seed, offset, shared_dim, out)

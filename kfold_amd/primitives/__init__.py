@@ -1,5 +1,6 @@
 """Module-level mirrors of the reference's hot-path primitives with ``kernel_backend="hip"``."""
 
+from .dropout import Dropout  # noqa: F401
 from .layers import LayerNorm, Linear, LinearNoBias  # noqa: F401
 from .triangle_multiplication import (  # noqa: F401
     TriangleMultiplicationIncoming,

@@ -1,11 +1,14 @@
 """Parameter holders with the reference's names (primitives/normalization.py:22,
-primitives/linear.py:22,110).  They own parameters only; the arithmetic of the hip backend
-lives in the fused kernels, which read these parameters through the packed-weight cache."""
+primitives/linear.py:22,110).  Inside the inference modules they own parameters only: the arithmetic
+lives in the fused kernels, which read these parameters through the packed-weight cache.
+``LayerNorm`` can also be called by itself (normalization.py:61-91), with gradients."""
 
 from __future__ import annotations
 
 import torch
 from torch import nn
+
+from .. import functional
 
 
 class LayerNorm(nn.Module):
@@ -16,6 +19,10 @@ class LayerNorm(nn.Module):
         self.eps = eps
         self.weight = nn.Parameter(torch.ones(normalized_shape)) if create_scale else None
         self.bias = nn.Parameter(torch.zeros(normalized_shape)) if create_offset else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """Layer norm over the last dim of x in fp32 statistics, result in x.dtype; differentiable."""
+        return functional.layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class Linear(nn.Module):
