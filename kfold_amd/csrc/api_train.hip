@@ -12,7 +12,7 @@ static bool misaligned(const void* p, size_t a = 16) { return (reinterpret_cast<
 
 // most rows / elements one call takes: grids and 64-bit offsets stay far from their ends
 static constexpr long long kMaxRows = 1LL << 29;
-static constexpr long long kMaxElems = 1LL << 36;
+static constexpr long long kMaxElems = 1LL << 34;
 
 extern "C" {
 
