@@ -403,8 +403,7 @@ int kfh_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, vo
                           size_t workspace_bytes, long long rows, int C, int F, int io_dtype, void* stream);
 
 /* Gradients for dy [rows, C]: dx [rows, C] (io_dtype), dw_in [2F, C] and dw_out [C, F] (dw_dtype);
- * each may be NULL.  u and v are computed again from x.  `dx` may be `dy`.  rows = 0 gives zero
- * weight gradients. */
+ * each may be NULL.  u and v are computed again from x.  rows = 0 gives zero weight gradients. */
 int kfh_gated_ffn_backward(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx,
                            void* dw_in, void* dw_out, int dw_dtype, void* workspace, size_t workspace_bytes,
                            long long rows, int C, int F, int io_dtype, void* stream);

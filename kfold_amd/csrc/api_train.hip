@@ -102,7 +102,7 @@ int kfh_gated_ffn_backward(const void* dy, const void* x, const void* w_in, cons
     if (!dy || !x || !w_in || !w_out) return fail(KFH_EINVAL, "gated_ffn_backward: null pointer argument");
     if (misaligned(dy) || misaligned(x) || misaligned(w_in) || misaligned(w_out) || misaligned(dx))
         return fail(KFH_EINVAL, "gated_ffn_backward: tensors must be aligned to 16 bytes");
-    if (dx && dx == x) return fail(KFH_EINVAL, "gated_ffn_backward: dx may alias dy, not x");
+    if (dx && (dx == x || dx == dy)) return fail(KFH_EINVAL, "gated_ffn_backward: dx must not alias x or dy");
     const size_t need = kfh_gated_ffn_workspace_bytes(rows, C, F, 1, io_dtype);
     if (!workspace || workspace_bytes < need || misaligned(workspace, 256))
         return fail(KFH_EINVAL, "gated_ffn_backward: workspace %zu bytes, need %zu aligned to 256",

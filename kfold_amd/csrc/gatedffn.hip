@@ -20,15 +20,33 @@ namespace kfh {
 
 // ---------------------------------------------------------------------------------------------
 // Operand tiles.  A tile of ROWS x BK operand values (rows: output index, k: contraction) goes
-// from memory to registers to LDS, where it is stored [part][row][BK + 8] bf16, so that the 8
-// k-consecutive values of an MFMA fragment are one 16-byte read; the 8 values of padding keep
-// consecutive rows on different banks.
+// from memory to registers (fetch) to LDS (commit), where it is stored [part][row][BK + 8] bf16, so
+// that the 8 k-consecutive values of an MFMA fragment are one 16-byte read; the 8 values of padding
+// keep consecutive rows on different banks.
 //   KC = true : memory is [row][k], k contiguous: a thread moves 8 k of a row
 //   KC = false: memory is [k][row], rows contiguous: a thread loads 4 k x 8 rows and writes them
 //               transposed, 4 k (8 bytes) per row
-// Values outside [row < rmax, k < kmax] are zeros.
+// Values outside [row < rmax, k < kmax] are zeros: the addresses are clamped into the tensor, so that
+// no load sits behind a branch, and the values cleared when they are committed.
 // ---------------------------------------------------------------------------------------------
 template <int IO> constexpr int parts_of() { return IO == KFH_F32 ? 3 : 1; }
+
+template <int IO> struct Raw8;                               // 8 values as they come from memory
+template <> struct Raw8<KFH_BF16> {
+    u32x4 w;
+    __device__ __forceinline__ void get(const void* p, size_t e) { w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + e); }
+    __device__ __forceinline__ void clear() { w = u32x4{0u, 0u, 0u, 0u}; }
+};
+template <> struct Raw8<KFH_F32> {
+    f32x4 a, b;
+    __device__ __forceinline__ void get(const void* p, size_t e) {
+        const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + e);
+        a = s[0];
+        b = s[1];
+    }
+    __device__ __forceinline__ void clear() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ float at(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
+};
 
 template <int IO, bool KC, int ROWS, int BK>
 struct TileLoad {
@@ -38,49 +56,49 @@ struct TileLoad {
     static constexpr int UNITS = KC ? ROWS * BK / 8 : ROWS * BK / 32;
     static constexpr int NU = (UNITS + 255) / 256;           // units per thread
     static constexpr int NV = KC ? 1 : 4;                    // 8-value vectors per unit
-    float v[NU][NV][8];
+    Raw8<IO> v[NU][NV];
+    unsigned bad;                                            // bit i * NV + j: vector j of unit i lies outside
 
-    __device__ __forceinline__ void load(const void* src, long long ld, long long row0, long long rmax,
-                                         long long k0, long long kmax, int tid) {
+    __device__ __forceinline__ void fetch(const void* src, long long ld, long long row0, long long rmax,
+                                          long long k0, long long kmax, int tid) {
+        bad = 0;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             const int u = i * 256 + tid;
             if constexpr (KC) {
                 const long long r = row0 + u / (BK / 8), k = k0 + (u % (BK / 8)) * 8;
-                const bool ok = u < UNITS && r < rmax && k < kmax;
-                if (ok) load8<IO>(src, (size_t)(r * ld + k), v[i][0]);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][0][e] = 0.f;
+                bad |= (unsigned)(r >= rmax || k >= kmax) << i;
+                v[i][0].get(src, (size_t)(min(r, rmax - 1) * ld + min(k, kmax - 8)));
             } else {
                 const long long r = row0 + (u / (BK / 4)) * 8, k = k0 + (u % (BK / 4)) * 4;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const bool ok = u < UNITS && r < rmax && k + j < kmax;
-                    if (ok) load8<IO>(src, (size_t)((k + j) * ld + r), v[i][j]);
-                    else
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[i][j][e] = 0.f;
+                    bad |= (unsigned)(r >= rmax || k + j >= kmax) << (4 * i + j);
+                    v[i][j].get(src, (size_t)(min(k + j, kmax - 1) * ld + min(r, rmax - 8)));
                 }
             }
         }
     }
-    __device__ __forceinline__ void store(uint16_t* lds, int tid) const {
+    __device__ __forceinline__ void commit(uint16_t* lds, int tid) {
+        if (bad) {
+#pragma unroll
+            for (int i = 0; i < NU; ++i)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if ((bad >> (i * NV + j)) & 1) v[i][j].clear();
+        }
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             const int u = i * 256 + tid;
-            if (u >= UNITS) continue;
+            if (UNITS % 256 != 0 && u >= UNITS) continue;
             if constexpr (KC) {
                 uint16_t* d = lds + (u / (BK / 8)) * LDK + (u % (BK / 8)) * 8;
                 if constexpr (PARTS == 1) {
-                    u32x4 w;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[i][0][2 * e], v[i][0][2 * e + 1]);
-                    *reinterpret_cast<u32x4*>(d) = w;
+                    *reinterpret_cast<u32x4*>(d) = v[i][0].w;
                 } else {
                     float q[8][3];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) split3(v[i][0][e], q[e]);
+                    for (int e = 0; e < 8; ++e) split3(v[i][0].at(e), q[e]);
 #pragma unroll
                     for (int p = 0; p < 3; ++p) {
                         u32x4 w;
@@ -94,12 +112,15 @@ struct TileLoad {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if constexpr (PARTS == 1) {
-                        u32x2 w = {pack_bf16(v[i][0][e], v[i][1][e]), pack_bf16(v[i][2][e], v[i][3][e])};
+                        // half-word e of the four vectors
+                        const uint32_t a = v[i][0].w[e >> 1], b = v[i][1].w[e >> 1], c = v[i][2].w[e >> 1], f = v[i][3].w[e >> 1];
+                        const u32x2 w = (e & 1) ? u32x2{(a >> 16) | (b & 0xffff0000u), (c >> 16) | (f & 0xffff0000u)}
+                                                : u32x2{(a & 0xffffu) | (b << 16), (c & 0xffffu) | (f << 16)};
                         *reinterpret_cast<u32x2*>(d + e * LDK) = w;
                     } else {
                         float q[4][3];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) split3(v[i][j][e], q[j]);
+                        for (int j = 0; j < 4; ++j) split3(v[i][j].at(e), q[j]);
 #pragma unroll
                         for (int p = 0; p < 3; ++p) {
                             u32x2 w = {pack_bf16(q[0][p], q[1][p]), pack_bf16(q[2][p], q[3][p])};
@@ -167,193 +188,630 @@ __device__ __forceinline__ void store4(void* base, size_t e, float a, float b, f
     else *reinterpret_cast<f32x4*>(static_cast<float*>(base) + e) = f32x4{a, b, c, d};
 }
 
+// Workgroups are dealt to the 8 XCDs in turn, each with an L2 of its own: the `nt` tiles that share a
+// row tile follow each other on one XCD, so its rows are read from memory once.  With few row tiles
+// that would leave XCDs idle (one row tile: seven of them), and the tiles are simply counted through.
+constexpr long long kXcdRows = 64;
+__device__ __forceinline__ bool xcd_tile(long long id, long long mtiles, int nt, long long& mt, int& n) {
+    const long long slot = mtiles >= kXcdRows ? id >> 3 : id;
+    mt = slot / nt;
+    n = (int)(slot - mt * nt);
+    if (mtiles >= kXcdRows) mt = mt * 8 + (id & 7);
+    return mt < mtiles;
+}
+static unsigned xcd_grid(long long mtiles, int nt) {
+    return (unsigned)((mtiles >= kXcdRows ? (mtiles + 7) / 8 * 8 : mtiles) * nt);
+}
+
+// A finished tile of RM rows x RN columns goes through LDS so that it leaves in whole rows (16 bytes a
+// lane, 2 RN bytes a row) instead of 8 bytes of 64 different rows.  put: four consecutive columns.
+template <int IO, int RM, int RN>
+struct TileStore {
+    static constexpr int ES = IO == KFH_F32 ? 4 : 2;
+    static constexpr int LD = RN * ES + 16;                  // bytes per staged row
+    static constexpr int BYTES = RM * LD;
+    static __device__ __forceinline__ void put(char* t, int r, int c, float a, float b, float d, float e) {
+        store4<IO>(t + r * LD, (size_t)c, a, b, d, e);
+    }
+    static __device__ __forceinline__ void flush(const char* t, void* out, long long ld, long long m0, long long M, int n0,
+                                                 int N, int tid) {
+        constexpr int PER = RN * ES / 16;                    // 16-byte pieces per row
+#pragma unroll
+        for (int i = 0; i < RM * PER / 256; ++i) {
+            const int u = i * 256 + tid, r = u / PER, c = (u % PER) * (16 / ES);
+            if (m0 + r < M && n0 + c < N)
+                *reinterpret_cast<u32x4*>(static_cast<char*>(out) + ((size_t)(m0 + r) * ld + n0 + c) * ES) =
+                    *reinterpret_cast<const u32x4*>(t + r * LD + c * ES);
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------------------------
-// Hidden values of a tile of 64 rows x 64 hidden channels; wavefront (wm, wn) owns 32 x 32.
+// Hidden values of a tile of TM rows x 64 hidden channels; wavefront (wm, wn) owns TM / 2 rows x 32
+// channels of u and v (and dh: the same accumulator shape, from dy and w_out).
 //   forward : h [M, F]
 //   backward: d [M, 2F] = (du, dv) and h [M, F]
+// The next k-tile travels from memory while the matrix cores work on the present one.
 // ---------------------------------------------------------------------------------------------
-template <int IO, bool BWD>
+template <int IO, int TM> constexpr int hidden_lds(bool bwd) {
+    constexpr int BK = IO == KFH_F32 ? 32 : 64;
+    const int in = parts_of<IO>() * (TM + 128) * (BK + 8) * 2;
+    const int out = (bwd ? 3 : 1) * TileStore<IO, TM, 64>::BYTES;
+    return in > out ? in : out;
+}
+
+template <int IO, bool BWD, int TM>
 __global__ __launch_bounds__(256) void ffn_hidden_kernel(const void* __restrict__ x, const void* __restrict__ dy,
                                                          const void* __restrict__ w_in,
                                                          const void* __restrict__ w_out, void* __restrict__ h,
                                                          void* __restrict__ d, long long M, int C, int F) {
-    constexpr int BK = IO == KFH_F32 ? 32 : 64, LDK = BK + 8, T = 64;
-    constexpr int TILE = parts_of<IO>() * T * LDK;
-    __shared__ __attribute__((aligned(16))) uint16_t smem[3 * TILE];
+    constexpr int BK = IO == KFH_F32 ? 32 : 64, LDK = BK + 8, P = parts_of<IO>(), NA = TM / 64;
+    __shared__ __attribute__((aligned(16))) char smem[hidden_lds<IO, TM>(BWD)];
+    uint16_t* const sa = reinterpret_cast<uint16_t*>(smem);
+    uint16_t* const su = sa + P * TM * LDK;
+    uint16_t* const sv = su + P * 64 * LDK;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave & 1, wn = wave >> 1;
-    const long long m0 = (long long)blockIdx.x * T;
-    const int f0 = blockIdx.y * T;
-    f32x16 u[1][1], v[1][1], g[1][1];
+    long long mt;
+    int ft;
+    if (!xcd_tile(blockIdx.x, (M + TM - 1) / TM, (F + 63) / 64, mt, ft)) return;
+    const long long m0 = mt * TM;
+    const int f0 = ft * 64;
+    f32x16 u[NA][1], v[NA][1], g[NA][1];
     zero_acc(u); zero_acc(v); zero_acc(g);
-    TileLoad<IO, true, T, BK> lx, lu, lv;
+    TileLoad<IO, true, TM, BK> lx;
+    TileLoad<IO, true, 64, BK> lu, lv;
+    TileLoad<IO, false, 64, BK> lo;
+    lx.fetch(x, C, m0, M, 0, C, tid);
+    lu.fetch(w_in, C, f0, F, 0, C, tid);
+    lv.fetch(w_in, C, (long long)F + f0, 2LL * F, 0, C, tid);
     for (int k0 = 0; k0 < C; k0 += BK) {
-        lx.load(x, C, m0, M, k0, C, tid);
-        lu.load(w_in, C, f0, F, k0, C, tid);
-        lv.load(w_in, C, (long long)F + f0, 2LL * F, k0, C, tid);
         __syncthreads();
-        lx.store(smem, tid); lu.store(smem + TILE, tid); lv.store(smem + 2 * TILE, tid);
+        lx.commit(sa, tid); lu.commit(su, tid); lv.commit(sv, tid);
         __syncthreads();
-        tile_mma<IO, 1, 1, T, T, BK>(smem, wm * 32, smem + TILE, wn * 32, lane, u);
-        tile_mma<IO, 1, 1, T, T, BK>(smem, wm * 32, smem + 2 * TILE, wn * 32, lane, v);
+        if (k0 + BK < C) {
+            lx.fetch(x, C, m0, M, k0 + BK, C, tid);
+            lu.fetch(w_in, C, f0, F, k0 + BK, C, tid);
+            lv.fetch(w_in, C, (long long)F + f0, 2LL * F, k0 + BK, C, tid);
+        } else if (BWD) {
+            lx.fetch(dy, C, m0, M, 0, C, tid);
+            lo.fetch(w_out, F, f0, F, 0, C, tid);
+        }
+        tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), su, wn * 32, lane, u);
+        tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), sv, wn * 32, lane, v);
     }
     if constexpr (BWD) {
-        TileLoad<IO, false, T, BK> lo;
         for (int k0 = 0; k0 < C; k0 += BK) {
-            lx.load(dy, C, m0, M, k0, C, tid);
-            lo.load(w_out, F, f0, F, k0, C, tid);
             __syncthreads();
-            lx.store(smem, tid); lo.store(smem + TILE, tid);
+            lx.commit(sa, tid); lo.commit(su, tid);
             __syncthreads();
-            tile_mma<IO, 1, 1, T, T, BK>(smem, wm * 32, smem + TILE, wn * 32, lane, g);
+            if (k0 + BK < C) {
+                lx.fetch(dy, C, m0, M, k0 + BK, C, tid);
+                lo.fetch(w_out, F, f0, F, k0 + BK, C, tid);
+            }
+            tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), su, wn * 32, lane, g);
         }
     }
-    const long long m = m0 + wm * 32 + (lane & 31);
-    if (m >= M) return;
+    __syncthreads();
+    using Out = TileStore<IO, TM, 64>;
+    char* const th = smem;
+    char* const tu = smem + Out::BYTES;
+    char* const tv = smem + 2 * Out::BYTES;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int f = f0 + wn * 32 + 8 * q + 4 * (lane >> 5);
-        if (f >= F) continue;
-        float hh[4], du[4], dv[4];
+    for (int a = 0; a < NA; ++a) {
+        const int r = wm * (TM / 2) + 32 * a + (lane & 31);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float uu = u[0][0][4 * q + e], vv = v[0][0][4 * q + e];
-            const float s = sigmoidf_fast(uu), us = uu * s;
-            hh[e] = us * vv;
+        for (int q = 0; q < 4; ++q) {
+            const int f = wn * 32 + 8 * q + 4 * (lane >> 5);
+            float hh[4], du[4], dv[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float uu = u[a][0][4 * q + e], vv = v[a][0][4 * q + e];
+                const float s = sigmoidf_fast(uu), us = uu * s;
+                hh[e] = us * vv;
+                if constexpr (BWD) {
+                    const float gg = g[a][0][4 * q + e];
+                    dv[e] = gg * us;
+                    du[e] = gg * vv * (s + us * (1.f - s));
+                }
+            }
+            Out::put(th, r, f, hh[0], hh[1], hh[2], hh[3]);
             if constexpr (BWD) {
-                const float gg = g[0][0][4 * q + e];
-                dv[e] = gg * us;
-                du[e] = gg * vv * (s + us * (1.f - s));
+                Out::put(tu, r, f, du[0], du[1], du[2], du[3]);
+                Out::put(tv, r, f, dv[0], dv[1], dv[2], dv[3]);
             }
         }
-        store4<IO>(h, (size_t)m * F + f, hh[0], hh[1], hh[2], hh[3]);
-        if constexpr (BWD) {
-            store4<IO>(d, (size_t)m * 2 * F + f, du[0], du[1], du[2], du[3]);
-            store4<IO>(d, (size_t)m * 2 * F + F + f, dv[0], dv[1], dv[2], dv[3]);
-        }
+    }
+    __syncthreads();
+    Out::flush(th, h, F, m0, M, f0, F, tid);
+    if constexpr (BWD) {
+        Out::flush(tu, d, 2LL * F, m0, M, f0, F, tid);
+        Out::flush(tv, static_cast<char*>(d) + (size_t)F * Out::ES, 2LL * F, m0, M, f0, F, tid);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// out[m][n] = sum_k A(m, k) B(n, k); AKC / BKC as TileLoad's KC.  blockIdx.z takes the contraction
-// range [z * kper, (z + 1) * kper); with SPLIT the result is an fp32 partial tile at
-// out + z * Mo * No, else it is written as IO.
+// out[m][n] = sum_k A(m, k) B(n, k); AKC / BKC as TileLoad's KC; a workgroup owns T x T results, a
+// wavefront T/2 x T/2.  The contraction is cut into `splits` ranges of kper; with more than one the
+// results are fp32 partial tiles at out + range * Mo * No (PART), else they are written as IO.
 // ---------------------------------------------------------------------------------------------
-template <int IO, bool AKC, bool BKC, bool SPLIT>
+template <int IO, int T> constexpr int gemm_lds(bool part) {
+    constexpr int BK = IO == KFH_F32 ? 32 : 64;
+    const int in = 2 * parts_of<IO>() * 2 * T * (BK + 8) * 2;
+    const int out = part ? TileStore<KFH_F32, T, T / 2>::BYTES : TileStore<IO, T, T / 2>::BYTES;
+    return in > out ? in : out;
+}
+
+template <int IO, bool AKC, bool BKC, bool PART, int T>
 __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ A, long long lda,
                                                        const void* __restrict__ B, long long ldb, void* __restrict__ out,
-                                                       long long Mo, int No, long long K, long long kper) {
-    constexpr int BK = IO == KFH_F32 ? 32 : 64, LDK = BK + 8, T = 64;
-    constexpr int TILE = parts_of<IO>() * T * LDK;
-    __shared__ __attribute__((aligned(16))) uint16_t smem[2 * TILE];
+                                                       long long Mo, int No, long long K, long long kper, int splits) {
+    constexpr int BK = IO == KFH_F32 ? 32 : 64, LDK = BK + 8, P = parts_of<IO>(), NA = T / 64;
+    __shared__ __attribute__((aligned(16))) char smem[gemm_lds<IO, T>(PART)];
+    constexpr int BUF = 2 * P * T * LDK;
+    uint16_t* const buf = reinterpret_cast<uint16_t*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave & 1, wn = wave >> 1;
-    const long long m0 = (long long)blockIdx.x * T;
-    const int n0 = blockIdx.y * T;
-    const long long kb = (long long)blockIdx.z * kper, ke = min(kb + kper, K);
-    f32x16 acc[1][1];
+    const long long mtiles = (Mo + T - 1) / T;
+    const int ntiles = (No + T - 1) / T;
+    // tiles that share operand rows follow each other on one XCD: those of a row tile, or (PART) all
+    // tiles of one range of the contraction
+    long long mt, z = 0;
+    int nt;
+    if constexpr (PART) {
+        int t;
+        if (!xcd_tile(blockIdx.x, splits, (int)(mtiles * ntiles), z, t)) return;
+        mt = t / ntiles;
+        nt = t % ntiles;
+    } else {
+        if (!xcd_tile(blockIdx.x, mtiles, ntiles, mt, nt)) return;
+    }
+    const long long m0 = mt * T;
+    const int n0 = nt * T;
+    const long long kb = z * kper, ke = min(kb + kper, K);
+    f32x16 acc[NA][NA];
     zero_acc(acc);
     TileLoad<IO, AKC, T, BK> la;
     TileLoad<IO, BKC, T, BK> lb;
-    for (long long k0 = kb; k0 < ke; k0 += BK) {
-        la.load(A, lda, m0, Mo, k0, ke, tid);
-        lb.load(B, ldb, n0, No, k0, ke, tid);
+    // two k-tiles ahead: while the matrix cores work on one from LDS, the next is written to the other LDS
+    // buffer and the one after travels from memory to registers; one barrier per k-tile
+    const long long steps = kb < ke ? (ke - kb + BK - 1) / BK : 0;
+    auto fetch = [&](long long s) {
+        if (s >= steps) return;
+        la.fetch(A, lda, m0, Mo, kb + s * BK, ke, tid);
+        lb.fetch(B, ldb, n0, No, kb + s * BK, ke, tid);
+    };
+    auto commit = [&](long long s) {
+        if (s >= steps) return;
+        uint16_t* const b = buf + (s & 1) * BUF;
+        la.commit(b, tid);
+        lb.commit(b + P * T * LDK, tid);
+    };
+    fetch(0);
+    commit(0);
+    fetch(1);
+    __syncthreads();
+    for (long long s = 0; s < steps; ++s) {
+        commit(s + 1);
+        fetch(s + 2);
+        const uint16_t* const b = buf + (s & 1) * BUF;
+        tile_mma<IO, NA, NA, T, T, BK>(b, wm * (T / 2), b + P * T * LDK, wn * (T / 2), lane, acc);
         __syncthreads();
-        la.store(smem, tid); lb.store(smem + TILE, tid);
-        __syncthreads();
-        tile_mma<IO, 1, 1, T, T, BK>(smem, wm * 32, smem + TILE, wn * 32, lane, acc);
     }
-    const long long m = m0 + wm * 32 + (lane & 31);
-    if (m >= Mo) return;
+    // through LDS in two halves of T / 2 columns
+    constexpr int OIO = PART ? KFH_F32 : IO;
+    using Out = TileStore<OIO, T, T / 2>;
+    char* const base = static_cast<char*>(out) + (PART ? (size_t)z * Mo * No * 4 : 0);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn * 32 + 8 * q + 4 * (lane >> 5);
-        if (n >= No) continue;
-        const f32x16& a = acc[0][0];
-        if constexpr (SPLIT)
-            store4<KFH_F32>(out, ((size_t)blockIdx.z * Mo + m) * No + n, a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
-        else
-            store4<IO>(out, (size_t)m * No + n, a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
+    for (int half = 0; half < 2; ++half) {
+        if (half) __syncthreads();
+        if (wn == half) {
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+#pragma unroll
+                for (int b = 0; b < NA; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        Out::put(smem, wm * (T / 2) + 32 * a + (lane & 31), 32 * b + 8 * q + 4 * (lane >> 5), acc[a][b][4 * q],
+                                 acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
+        }
+        __syncthreads();
+        Out::flush(smem, base, No, m0, Mo, n0 + half * (T / 2), No, tid);
     }
 }
 
-// out[i] = sum of `parts` fp32 values part[z * n + i], in order
+// out[i] = sum of `parts` fp32 values part[z * n + i]: 64 lanes x 4 values per workgroup, its four
+// wavefronts take every fourth part; a fixed order
 __global__ __launch_bounds__(256) void ffn_sum_parts_kernel(const float* __restrict__ part, int parts, long long n,
                                                             void* __restrict__ out, int out_dtype) {
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
+    __shared__ f32x4 red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long i = ((long long)blockIdx.x * 64 + lane) * 4;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < parts; ++z) {
-        const f32x4 w = *reinterpret_cast<const f32x4*>(part + (size_t)z * n + i);
+    if (i < n) {
+#pragma unroll 4
+        for (int z = wave; z < parts; z += 4) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(part + (size_t)z * n + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += w[e];
+            for (int e = 0; e < 4; ++e) s[e] += w[e];
+        }
     }
-    if (out_dtype == KFH_BF16) store4<KFH_BF16>(out, (size_t)i, s[0], s[1], s[2], s[3]);
-    else store4<KFH_F32>(out, (size_t)i, s[0], s[1], s[2], s[3]);
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || i >= n) return;
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (red[0][lane][e] + red[1][lane][e]) + (red[2][lane][e] + red[3][lane][e]);
+    if (out_dtype == KFH_BF16) store4<KFH_BF16>(out, (size_t)i, o[0], o[1], o[2], o[3]);
+    else store4<KFH_F32>(out, (size_t)i, o[0], o[1], o[2], o[3]);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows of C = 64, 128 or 256 channels in bf16 (the pair track's widths): rows stay, weights
+// stream.  A wavefront holds the MFMA fragments of 32 rows of x (and dy) in registers for the whole
+// kernel; each step brings the weights of 32 hidden channels, packed as MFMA fragments, through
+// double-buffered LDS and computes u, v (and dh) as D[hidden][row].  The rounded accumulators are by
+// themselves the row operand of the next product (K_ACC order), so
+//   forward,  FUSE: y += h W_out^T stays in registers, h never leaves them
+//   backward, FUSE: dx += [du dv] W_in likewise; du, dv and h are written for the weight gradients
+// FUSE needs C / 2 accumulator registers more, which C = 256 does not have; there the second product
+// is a launch of its own.  Bound by the LDS reads of the weights (one 1 KiB fragment per MFMA) and the
+// activation's VALU work.
+// ---------------------------------------------------------------------------------------------
+template <int KS, bool BWD, bool FUSE> constexpr int stream_frags() {
+    return (BWD ? 3 : 2) * KS + (FUSE ? (BWD ? 2 : 1) * KS : 0);
+}
+// output channel of accumulator block n, column col: NI adjacent channels per lane
+template <int KS> __host__ __device__ constexpr int stream_chan(int n, int col) {
+    constexpr int NI = KS / 2 < 4 ? KS / 2 : 4;
+    return (n / NI) * 32 * NI + NI * col + n % NI;
+}
+
+// Packed weights of a step of 32 hidden channels f0.., 1 KiB per fragment, lane-major:
+//   KS x W_in rows f0.. (u), KS x W_in rows F + f0.. (v), [BWD] KS x W_out columns f0.. (dh),
+//   [FUSE] forward: KS x W_out as B operand (block n, k-step); backward: KS x W_in u rows, KS x v rows
+template <int KS, bool BWD, bool FUSE>
+__global__ __launch_bounds__(256) void ffn_pack_kernel(const uint16_t* __restrict__ w_in, const uint16_t* __restrict__ w_out,
+                                                       u32x4* __restrict__ dst, int F, long long slots) {
+    constexpr int C = 16 * KS, NF = stream_frags<KS, BWD, FUSE>();
+    const long long slot = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (slot >= slots) return;
+    const int lane = (int)(slot & 63), fr = (int)((slot >> 6) % NF);
+    const int f0 = (int)((slot >> 6) / NF) * 32, col = lane & 31, half = lane >> 5;
+    const int group = fr / KS, ks = fr % KS;
+    uint32_t v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int c = 16 * ks + 8 * half + e;                           // contraction over channels
+        const int f = f0 + 16 * (ks & 1) + 8 * (e >> 2) + 4 * half + (e & 3);    // over hidden (K_ACC)
+        size_t src;
+        const uint16_t* w = w_in;
+        if (group < 2) src = (size_t)(group * F + f0 + col) * C + c;
+        else if (BWD && group == 2) { w = w_out; src = (size_t)c * F + f0 + col; }
+        else if (!BWD) { w = w_out; src = (size_t)stream_chan<KS>(ks >> 1, col) * F + f; }
+        else src = (size_t)((group - 3) * F + f) * C + stream_chan<KS>(ks >> 1, col);
+        v[e] = w[src];
+    }
+    dst[slot] = u32x4{v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16), v[6] | (v[7] << 16)};
+}
+
+// two fragments of D[hidden][row] values -> row `p` of a row-major tensor: the halves of the wavefront
+// trade 4-channel groups, so that a lane stores 8 consecutive channels (16 bytes)
+__device__ __forceinline__ void store_hidden(uint16_t* row, int half, bool live, const bf16x8& f0, const bf16x8& f1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const u32x4 w = __builtin_bit_cast(u32x4, i ? f1 : f0);
+        const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        if (live) *reinterpret_cast<u32x4*>(row + 16 * i + 8 * half) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+}
+
+template <int KS, bool BWD, bool FUSE, int NW, int OCC>
+__global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t* __restrict__ x,
+                                                                  const uint16_t* __restrict__ dy,
+                                                                  const u32x4* __restrict__ wp, uint16_t* __restrict__ h,
+                                                                  uint16_t* __restrict__ d, uint16_t* __restrict__ out, long long M,
+                                                                  int F, int steps_per) {
+    constexpr int C = 16 * KS, NF = stream_frags<KS, BWD, FUSE>(), NT = NW * 64, NB = FUSE ? KS / 2 : 1;
+    constexpr int SLOTS = NF * 64, NPRE = (SLOTS + NT - 1) / NT;
+    __shared__ __attribute__((aligned(16))) u32x4 smem[2 * SLOTS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    const long long p0 = (long long)blockIdx.x * (32 * NW) + wave * 32;
+    const int s0 = blockIdx.y * steps_per, s1 = min(s0 + steps_per, F / 32);
+    u32x4 pre[NPRE];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < NPRE; ++i) pre[i] = wp[(size_t)s * SLOTS + min(i * NT + tid, SLOTS - 1)];
+    };
+    auto commit = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < NPRE; ++i)
+            if (SLOTS % NT == 0 || i * NT + tid < SLOTS) smem[b * SLOTS + i * NT + tid] = pre[i];
+    };
+    fetch(s0);
+    const long long p = p0 + col;
+    const bool live = p < M;
+    const size_t row = (size_t)min(p, M - 1) * C + 8 * half;
+    bf16x8 xf[KS], yf[BWD ? KS : 1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) xf[ks] = *reinterpret_cast<const bf16x8*>(x + row + 16 * ks);
+    if constexpr (BWD) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) yf[ks] = *reinterpret_cast<const bf16x8*>(dy + row + 16 * ks);
+    }
+    commit(0);
+    __syncthreads();
+    f32x16 oacc[NB];
+    if constexpr (FUSE) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) oacc[n][v] = 0.f;
+    }
+    for (int s = s0; s < s1; ++s) {
+        if (s + 1 < s1) fetch(s + 1);
+        const bf16x8* w = reinterpret_cast<const bf16x8*>(smem + ((s - s0) & 1) * SLOTS) + lane;
+        f32x16 u, v, g;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { u[i] = 0.f; v[i] = 0.f; g[i] = 0.f; }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            u = mfma32(w[ks * 64], xf[ks], u);
+            v = mfma32(w[(KS + ks) * 64], xf[ks], v);
+            if constexpr (BWD) g = mfma32(w[(2 * KS + ks) * 64], yf[ks], g);
+        }
+        const size_t hrow = (size_t)p * F + s * 32;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float sg = sigmoidf_fast(u[i]), us = u[i] * sg;
+            if constexpr (BWD) {
+                const float gg = g[i], vv = v[i];
+                g[i] = us * vv;                                          // h
+                u[i] = gg * vv * (sg + us * (1.f - sg));                 // du
+                v[i] = gg * us;                                          // dv
+            } else {
+                u[i] = us * v[i];                                        // h
+            }
+        }
+        bf16x8 a0, a1;
+        if constexpr (BWD) {
+            bf16x8 b0, b1, h0, h1;
+            acc_to_frags(u, a0, a1);
+            acc_to_frags(v, b0, b1);
+            acc_to_frags(g, h0, h1);
+            if constexpr (FUSE) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    oacc[n] = mfma32(a0, w[(3 * KS + 2 * n) * 64], oacc[n]);
+                    oacc[n] = mfma32(a1, w[(3 * KS + 2 * n + 1) * 64], oacc[n]);
+                    oacc[n] = mfma32(b0, w[(4 * KS + 2 * n) * 64], oacc[n]);
+                    oacc[n] = mfma32(b1, w[(4 * KS + 2 * n + 1) * 64], oacc[n]);
+                }
+            }
+            store_hidden(h + hrow, half, live, h0, h1);
+            store_hidden(d + 2 * hrow - s * 32, half, live, a0, a1);
+            store_hidden(d + 2 * hrow - s * 32 + F, half, live, b0, b1);
+        } else {
+            acc_to_frags(u, a0, a1);
+            if constexpr (FUSE) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    oacc[n] = mfma32(a0, w[(2 * KS + 2 * n) * 64], oacc[n]);
+                    oacc[n] = mfma32(a1, w[(2 * KS + 2 * n + 1) * 64], oacc[n]);
+                }
+            } else {
+                store_hidden(h + hrow, half, live, a0, a1);
+            }
+        }
+        if (s + 1 < s1) commit((s + 1 - s0) & 1);
+        __syncthreads();
+    }
+    if constexpr (FUSE) {
+        if (!out) return;                                                // no dx asked for
+        constexpr int NI = NB < 4 ? NB : 4;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const long long q = p0 + acc_row(v, half);
+            if (q >= M) continue;
+#pragma unroll
+            for (int n = 0; n < NB; n += NI) {
+                uint16_t* o = out + (size_t)q * C + stream_chan<KS>(n, col);
+                if constexpr (NI == 4)
+                    *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16(oacc[n][v], oacc[n + 1][v]), pack_bf16(oacc[n + 2][v], oacc[n + 3][v])};
+                else
+                    *reinterpret_cast<uint32_t*>(o) = pack_bf16(oacc[n][v], oacc[n + 1][v]);
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// ranges of rows the weight gradients are summed over in parallel: about 1024 workgroups, at least
-// 256 rows each
-static int wgrad_splits(long long M, long long tiles) {
-    const long long want = max(1LL, 1024 / max(1LL, tiles)), most = max(1LL, (M + 255) / 256);
-    return (int)min(min(want, most), 256LL);
+// Tiles of 128 x 128 feed the matrix cores twice as well as tiles of 64 x 64 but leave the chip empty
+// when there are few of them: they are taken when they give every CU a workgroup.
+static bool big_tiles(long long a, long long b, long long more = 1) { return up_div(a, 128) * up_div(b, 128) * more >= 256; }
+
+// Ranges of rows the weight gradients are summed over in parallel: four workgroups per CU, at least
+// 256 rows each.
+struct Wgrad { int T, splits; long long per; };
+static Wgrad wgrad_plan(long long M, long long a, long long b, int io_dtype) {
+    Wgrad w;
+    const long long most = max(1LL, up_div(M, 256));
+    w.T = io_dtype == KFH_BF16 && big_tiles(a, b, most) ? 128 : 64;
+    const long long tiles = up_div(a, w.T) * up_div(b, w.T);
+    w.splits = (int)min(min(max(1LL, 1024 / tiles), most), 256LL);
+    w.per = up_div(up_div(M, w.splits), 64) * 64;
+    return w;
 }
-static long long tiles64(long long a, long long b) { return ((a + 63) / 64) * ((b + 63) / 64); }
-static size_t wgrad_part_bytes(long long M, int C, int F) {
-    const size_t a = (size_t)wgrad_splits(M, tiles64(2 * F, C)) * 2 * F * C * 4;
-    const size_t b = (size_t)wgrad_splits(M, tiles64(C, F)) * F * C * 4;
+static size_t wgrad_part_bytes(long long M, int C, int F, int io_dtype) {
+    const size_t a = (size_t)wgrad_plan(M, 2LL * F, C, io_dtype).splits * 2 * F * C * 4;
+    const size_t b = (size_t)wgrad_plan(M, C, F, io_dtype).splits * F * C * 4;
     return a > b ? a : b;
 }
 
-size_t gated_ffn_ws_bytes(long long M, int C, int F, int backward, int io_dtype) {
+// A product with few tiles and a long contraction is cut into ranges of it (at least 8 k-tiles each, from
+// 24 on, towards two workgroups per CU): 666 x 384 with K = 1536 in fp32 took 90 us in one piece.
+static int product_splits(long long Mo, long long No, long long K, int io_dtype) {
+    const long long BK = io_dtype == KFH_F32 ? 32 : 64, steps = up_div(K, BK);
+    if (steps < 24) return 1;
+    const long long tiles = up_div(Mo, 64) * up_div(No, 64);
+    return (int)max(1LL, min(512 / tiles, steps / 8));
+}
+static size_t product_part_bytes(long long Mo, long long No, long long K, int io_dtype) {
+    const int s = product_splits(Mo, No, K, io_dtype);
+    return s > 1 ? (size_t)s * Mo * No * 4 : 0;
+}
+
+// The streamed kernels: bf16, a width they are built for, whole steps of hidden channels, and rows enough
+// to give every CU a workgroup (below that their 128 or 256 rows per workgroup leave CUs idle).
+static bool streamed(long long M, int C, int F, int io_dtype) {
+    return io_dtype == KFH_BF16 && (C == 64 || C == 128 || C == 256) && F % 32 == 0 && M >= 16384;
+}
+static size_t stream_pack_bytes(int C, int F, int backward) {
+    const int KS = C / 16, nf = (backward ? 3 : 2) * KS + (C <= 128 ? (backward ? 2 : 1) * KS : 0);
+    return (size_t)(F / 32) * nf * 1024;
+}
+
+// workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F]; packed weights of the
+// streamed kernels; partial sums
+struct FfnWs { size_t h, d, pack, part, total; };
+static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     const size_t e = io_dtype == KFH_F32 ? 4 : 2;
-    if (!backward) return up256((size_t)M * F * e);
-    return up256((size_t)M * F * e) + up256((size_t)M * 2 * F * e) + up256(wgrad_part_bytes(M, C, F));
+    const bool st = streamed(M, C, F, io_dtype), fused = st && C <= 128;
+    FfnWs w;
+    w.h = 0;
+    w.d = w.h + (backward || !fused ? up256((size_t)M * F * e) : 0);
+    w.pack = w.d + (backward ? up256((size_t)M * 2 * F * e) : 0);
+    w.part = w.pack + (st ? up256(stream_pack_bytes(C, F, backward)) : 0);
+    size_t part = fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype);
+    if (backward) part = max(part, wgrad_part_bytes(M, C, F, io_dtype));
+    w.total = w.part + up256(part);
+    return w;
+}
+size_t gated_ffn_ws_bytes(long long M, int C, int F, int backward, int io_dtype) {
+    return ffn_ws(M, C, F, backward, io_dtype).total;
+}
+
+static void sum_parts(const float* part, int parts, long long n, void* out, int out_dtype, hipStream_t stream) {
+    hipLaunchKernelGGL(ffn_sum_parts_kernel, dim3((unsigned)up_div(n, 256)), dim3(256), 0, stream, part, parts, n, out,
+                       out_dtype);
+}
+
+// (fp32 stays with the small tiles: its operands take three times the LDS)
+template <int IO, bool BWD>
+static void hidden(const void* x, const void* dy, const void* w_in, const void* w_out, void* h, void* d, long long M, int C,
+                   int F, hipStream_t stream) {
+    const int nt = (int)up_div(F, 64);
+    if constexpr (IO == KFH_BF16) {
+        if (up_div(M, 128) * nt >= 256) {
+            hipLaunchKernelGGL((ffn_hidden_kernel<IO, BWD, 128>), dim3(xcd_grid(up_div(M, 128), nt)), dim3(256), 0, stream, x,
+                               dy, w_in, w_out, h, d, M, C, F);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((ffn_hidden_kernel<IO, BWD, 64>), dim3(xcd_grid(up_div(M, 64), nt)), dim3(256), 0, stream, x, dy, w_in,
+                       w_out, h, d, M, C, F);
+}
+
+template <int IO, bool AKC, bool BKC, bool PART, int T>
+static void gemm(const void* A, long long lda, const void* B, long long ldb, void* out, long long Mo, int No, long long K,
+                 long long kper, int splits, hipStream_t stream) {
+    const long long mt = up_div(Mo, T), nt = up_div(No, T);
+    hipLaunchKernelGGL((ffn_gemm_kernel<IO, AKC, BKC, PART, T>),
+                       dim3(PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(256), 0, stream, A, lda, B,
+                       ldb, out, Mo, No, K, kper, splits);
+}
+
+// out [Mo, No] = A [Mo, K] times B, [No, K] or (BKC = false) [K, No]; part: product_part_bytes
+template <int IO, bool BKC>
+static void product(const void* A, long long lda, const void* B, long long ldb, void* out, float* part, long long Mo, int No,
+                    long long K, hipStream_t stream) {
+    const int splits = product_splits(Mo, No, K, IO);
+    if (splits > 1) {
+        const long long BK = IO == KFH_F32 ? 32 : 64, per = up_div(up_div(K, BK), splits) * BK;
+        gemm<IO, true, BKC, true, 64>(A, lda, B, ldb, part, Mo, No, K, per, splits, stream);
+        sum_parts(part, splits, Mo * No, out, IO, stream);
+        return;
+    }
+    if constexpr (IO == KFH_BF16) {
+        if (big_tiles(Mo, No)) {
+            gemm<IO, true, BKC, false, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
+            return;
+        }
+    }
+    gemm<IO, true, BKC, false, 64>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
+}
+
+// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]
+template <int IO>
+static void wgrad(const void* A, int Ma, const void* B, int Nb, float* part, void* out, int out_dtype, long long M,
+                  hipStream_t stream) {
+    const Wgrad w = wgrad_plan(M, Ma, Nb, IO);
+    bool done = false;
+    if constexpr (IO == KFH_BF16) {
+        if (w.T == 128) {
+            gemm<IO, false, false, true, 128>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+            done = true;
+        }
+    }
+    if (!done) gemm<IO, false, false, true, 64>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+    sum_parts(part, w.splits, (long long)Ma * Nb, out, out_dtype, stream);
+}
+
+// hidden values (and, up to C = 128, the second product) of a streamed call
+template <int KS, bool BWD>
+static void stream(const void* x, const void* dy, const void* w_in, const void* w_out, char* ws, const FfnWs& w, void* out,
+                   long long M, int F, hipStream_t stream) {
+    constexpr bool FUSE = KS <= 8;
+    constexpr int NW = KS == 16 ? 8 : 4, OCC = BWD || KS == 16 ? 2 : 3;
+    u32x4* pack = reinterpret_cast<u32x4*>(ws + w.pack);
+    const long long slots = (long long)(F / 32) * stream_frags<KS, BWD, FUSE>() * 64;
+    hipLaunchKernelGGL((ffn_pack_kernel<KS, BWD, FUSE>), dim3((unsigned)up_div(slots, 256)), dim3(256), 0, stream,
+                       static_cast<const uint16_t*>(w_in), static_cast<const uint16_t*>(w_out), pack, F, slots);
+    // without the second product the hidden channels can be dealt out as well: towards eight rounds of
+    // workgroups, so that the last, partly filled one costs little
+    const long long tiles = up_div(M, 32 * NW);
+    const int steps = F / 32, parts = FUSE ? 1 : (int)max(1LL, min(2048 / tiles, (long long)steps / 4));
+    const int per = (int)up_div(steps, parts);
+    hipLaunchKernelGGL((ffn_stream_kernel<KS, BWD, FUSE, NW, OCC>), dim3((unsigned)tiles, (unsigned)up_div(steps, per)), dim3(NW * 64),
+                       0, stream, static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(dy), pack,
+                       reinterpret_cast<uint16_t*>(ws + w.h), reinterpret_cast<uint16_t*>(ws + w.d), static_cast<uint16_t*>(out), M, F,
+                       per);
+}
+template <bool BWD>
+static void stream_by_width(int C, const void* x, const void* dy, const void* w_in, const void* w_out, char* ws,
+                            const FfnWs& w, void* out, long long M, int F, hipStream_t s) {
+    if (C == 64) stream<4, BWD>(x, dy, w_in, w_out, ws, w, out, M, F, s);
+    else if (C == 128) stream<8, BWD>(x, dy, w_in, w_out, ws, w, out, M, F, s);
+    else stream<16, BWD>(x, dy, w_in, w_out, ws, w, out, M, F, s);
 }
 
 template <int IO>
 static void forward_t(const void* x, const void* w_in, const void* w_out, void* y, char* ws, long long M, int C, int F,
                       hipStream_t stream) {
-    const dim3 block(256);
-    hipLaunchKernelGGL((ffn_hidden_kernel<IO, false>), dim3((unsigned)((M + 63) / 64), (unsigned)((F + 63) / 64)), block, 0,
-                       stream, x, nullptr, w_in, nullptr, ws, nullptr, M, C, F);
-    hipLaunchKernelGGL((ffn_gemm_kernel<IO, true, true, false>), dim3((unsigned)((M + 63) / 64), (unsigned)((C + 63) / 64)),
-                       block, 0, stream, ws, (long long)F, w_out, (long long)F, y, M, C, (long long)F, (long long)F);
-}
-
-template <int IO>
-static void wgrad(const void* A, int Ma, const void* B, int Nb, float* part, void* out, int out_dtype, long long M,
-                  hipStream_t stream) {
-    const int splits = wgrad_splits(M, tiles64(Ma, Nb));
-    long long per = (M + splits - 1) / splits;
-    per = (per + 63) / 64 * 64;
-    hipLaunchKernelGGL((ffn_gemm_kernel<IO, false, false, true>),
-                       dim3((unsigned)((Ma + 63) / 64), (unsigned)((Nb + 63) / 64), (unsigned)splits), dim3(256), 0, stream, A,
-                       (long long)Ma, B, (long long)Nb, part, (long long)Ma, Nb, M, per);
-    const long long n = (long long)Ma * Nb;
-    hipLaunchKernelGGL(ffn_sum_parts_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, part, splits, n,
-                       out, out_dtype);
+    const FfnWs w = ffn_ws(M, C, F, 0, IO);
+    const bool st = streamed(M, C, F, IO);
+    if (st) stream_by_width<false>(C, x, nullptr, w_in, w_out, ws, w, y, M, F, stream);
+    else hidden<IO, false>(x, nullptr, w_in, nullptr, ws + w.h, nullptr, M, C, F, stream);
+    if (!(st && C <= 128)) product<IO, true>(ws + w.h, F, w_out, F, y, reinterpret_cast<float*>(ws + w.part), M, C, F, stream);
 }
 
 template <int IO>
 static void backward_t(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx, void* dw_in,
                        void* dw_out, int dw_dtype, char* ws, long long M, int C, int F, hipStream_t stream) {
-    const size_t e = IO == KFH_F32 ? 4 : 2;
-    char* h = ws;
-    char* d = h + up256((size_t)M * F * e);
-    float* part = reinterpret_cast<float*>(d + up256((size_t)M * 2 * F * e));
-    const dim3 block(256);
-    hipLaunchKernelGGL((ffn_hidden_kernel<IO, true>), dim3((unsigned)((M + 63) / 64), (unsigned)((F + 63) / 64)), block, 0,
-                       stream, x, dy, w_in, w_out, h, d, M, C, F);
-    // dy is read before dx, which may be written over it
+    const FfnWs w = ffn_ws(M, C, F, 1, IO);
+    char* const h = ws + w.h;
+    char* const d = ws + w.d;
+    float* const part = reinterpret_cast<float*>(ws + w.part);
+    const bool st = streamed(M, C, F, IO);
+    if (st) stream_by_width<true>(C, x, dy, w_in, w_out, ws, w, dx, M, F, stream);
+    else hidden<IO, true>(x, dy, w_in, w_out, h, d, M, C, F, stream);
     if (dw_out) wgrad<IO>(dy, C, h, F, part, dw_out, dw_dtype, M, stream);
     if (dw_in) wgrad<IO>(d, 2 * F, x, C, part, dw_in, dw_dtype, M, stream);
-    if (dx)
-        hipLaunchKernelGGL((ffn_gemm_kernel<IO, true, false, false>), dim3((unsigned)((M + 63) / 64), (unsigned)((C + 63) / 64)),
-                           block, 0, stream, d, 2LL * F, w_in, (long long)C, dx, M, C, 2LL * F, 2LL * F);
+    if (dx && !(st && C <= 128)) product<IO, false>(d, 2LL * F, w_in, C, dx, part, M, C, 2LL * F, stream);
 }
 
 void launch_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, void* y, char* ws, long long M,

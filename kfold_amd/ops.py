@@ -700,7 +700,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_
                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """``(dx, dw_in, dw_out)`` of ``gated_ffn_forward`` for the gradient dy of its result (the hidden
     values are computed again from x); the weight gradients in ``dw_dtype`` (default: the weights'),
-    None for what is not needed.  ``out`` (for dx) may be dy."""
+    None for what is not needed.  ``out`` is for dx (not dy itself)."""
     dev = _require_cuda(dy, x, w_in, w_out, out)
     io = _io_dtype(x)
     rows, C, F = _ffn_shapes(x, w_in, w_out)

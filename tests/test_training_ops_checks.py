@@ -73,6 +73,7 @@ def test_gated_ffn_checks(env):
     _expect(lib, b(*ok, 0, p[7], need - 1, 10, 64, 64, 0, None), EINVAL, "workspace", str(need))
     _expect(lib, b(*ok, 7, p[7], need, 10, 64, 64, 0, None), EINVAL, "dw_dtype 7")
     _expect(lib, b(p[0], p[1], p[2], p[3], p[1], p[5], p[6], 0, p[7], need, 10, 64, 64, 0, None), EINVAL, "alias")
+    _expect(lib, b(p[0], p[1], p[2], p[3], p[0], p[5], p[6], 0, p[7], need, 10, 64, 64, 0, None), EINVAL, "alias")
     _expect(lib, b(p[0], p[1], p[2], p[3], p[4], p[5] + 8, p[6], 0, p[7], need, 10, 64, 64, 0, None), EINVAL, "16 bytes")
     _expect(lib, b(None, p[1], p[2], p[3], p[4], p[5], p[6], 0, p[7], need, 10, 64, 64, 0, None), EINVAL, "null")
     assert ws(589824, 128, 256, 1, 0) < 16 << 30

@@ -264,13 +264,25 @@ def test_gated_ffn_forward_and_backward(M, C, F, dtype):
     within(dwo, r["dw_out"], e["dw_out"], "dw_out")
     again = ops.gated_ffn_backward(dyd, xd, wi, wo)
     assert all(torch.equal(p, q) for p, q in zip(again, (dx, dwi, dwo)))
-    inplace = dyd.clone()
-    got = ops.gated_ffn_backward(inplace, xd, wi, wo, out=inplace)
-    assert got[0] is inplace and all(torch.equal(p, q) for p, q in zip(got, (dx, dwi, dwo)))
     only = ops.gated_ffn_backward(dyd, xd, wi, wo, need_dw=False)
     assert torch.equal(only[0], dx) and only[1] is None and only[2] is None
     only = ops.gated_ffn_backward(dyd, xd, wi, wo, need_dx=False)
     assert only[0] is None and torch.equal(only[1], dwi) and torch.equal(only[2], dwo)
+
+
+@pytest.mark.parametrize("M,C,F", [(33001, 24, 40), (32900, 8, 136), (16400, 64, 32), (16385, 64, 96), (16500, 128, 64),
+                                   (16384, 256, 160)])
+def test_gated_ffn_big_tiles(M, C, F):
+    """Enough rows for every kernel to take its large tiles, or for the kernels that keep the rows in
+    registers (C = 64, 128, 256), with ragged edges on all sides."""
+    print(f"case gated ffn big tiles {M} x {C} x {F}", flush=True)
+    x, w_in, w_out, dy = ffn_inputs(M, C, F, BF, 6)
+    r = ffn64(x, w_in, w_out, dy)
+    e = ffn_bounds(x, w_in, w_out, r, BF, dy)
+    xd, wi, wo, dyd = (t.to(DEV) for t in (x, w_in, w_out, dy))
+    within(ops.gated_ffn_forward(xd, wi, wo), r["y"], e["y"], "y")
+    for got, name in zip(ops.gated_ffn_backward(dyd, xd, wi, wo), ("dx", "dw_in", "dw_out")):
+        within(got, r[name], e[name], name)
 
 
 def test_gated_ffn_many_rows():
@@ -525,6 +537,9 @@ def test_training_ops_refusals():
         ops.gated_ffn_backward(x, x, w_in, w_out, dw_dtype=torch.float16)
     with pytest.raises(Exception, match="alias"):
         ops.gated_ffn_backward(x.clone(), x, w_in, w_out, out=x)
+    with pytest.raises(Exception, match="alias"):
+        dy = x.clone()
+        ops.gated_ffn_backward(dy, x, w_in, w_out, out=dy)
     with pytest.raises(ValueError, match="probability"):
         ops.dropout_forward(x, 1.5, 0)
     with pytest.raises(ValueError, match="probability"):
