@@ -23,10 +23,12 @@ namespace kfh {
 // from memory to registers (fetch) to LDS (commit), where it is stored [part][row][BK + 8] bf16, so
 // that the 8 k-consecutive values of an MFMA fragment are one 16-byte read; the 8 values of padding
 // keep consecutive rows on different banks.
-//   KC = true : memory is [row][k], k contiguous: a thread moves 8 k of a row
-//   KC = false: memory is [k][row], rows contiguous: a thread loads 4 k x 8 rows and writes them
-//               transposed, 4 k (8 bytes) per row
-// Values outside [row < rmax, k < kmax] are zeros: the addresses are clamped into the tensor, so that
+//   K_MAJOR : memory is [row][k], k contiguous: a thread moves 8 k of a row
+//   R_MAJOR : memory is [k][row], rows contiguous: a thread loads 4 k x 8 rows and writes them
+//             transposed, 4 k (8 bytes) per row
+//   K_BLOCK, R_BLOCK: the same two for hidden values written by ffn_stream_kernel, blocks of 32 rows x
+//             32 channels (ld: channels) of two MFMA fragments each: hidden_slot
+// Values outside [row < rmax, k < kmax] are zeros: their addresses are kept inside the tensor, so that
 // no load sits behind a branch, and the values cleared when they are committed.
 // ---------------------------------------------------------------------------------------------
 template <int IO> constexpr int parts_of() { return IO == KFH_F32 ? 3 : 1; }
@@ -34,13 +36,13 @@ template <int IO> constexpr int parts_of() { return IO == KFH_F32 ? 3 : 1; }
 template <int IO> struct Raw8;                               // 8 values as they come from memory
 template <> struct Raw8<KFH_BF16> {
     u32x4 w;
-    __device__ __forceinline__ void get(const void* p, size_t e) { w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + e); }
+    __device__ __forceinline__ void get(const char* p, uint32_t o) { w = *reinterpret_cast<const u32x4*>(p + o); }
     __device__ __forceinline__ void clear() { w = u32x4{0u, 0u, 0u, 0u}; }
 };
 template <> struct Raw8<KFH_F32> {
     f32x4 a, b;
-    __device__ __forceinline__ void get(const void* p, size_t e) {
-        const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + e);
+    __device__ __forceinline__ void get(const char* p, uint32_t o) {
+        const f32x4* s = reinterpret_cast<const f32x4*>(p + o);
         a = s[0];
         b = s[1];
     }
@@ -48,33 +50,84 @@ template <> struct Raw8<KFH_F32> {
     __device__ __forceinline__ float at(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
 };
 
-template <int IO, bool KC, int ROWS, int BK>
+enum : int { K_MAJOR = 0, R_MAJOR, K_BLOCK, R_BLOCK };
+
+// 16-byte slot of the 8 channels 16 ks + 4 half + {0..3, 8..11} of block (m / 32, channel block hb), row m
+__device__ __forceinline__ size_t hidden_slot(long long m, int hb, int nhb, int ks, int half) {
+    return ((size_t)((m >> 5) * nhb + hb) * 2 + ks) * 64 + half * 32 + (m & 31);
+}
+
+template <int IO, int KIND, int ROWS, int BK>
 struct TileLoad {
+    static constexpr bool KC = KIND == K_MAJOR || KIND == K_BLOCK;
     static constexpr int PARTS = parts_of<IO>();
     static constexpr int LDK = BK + 8;                       // bf16 per stored row
     static constexpr int PLANE = ROWS * LDK;                 // bf16 per part
     static constexpr int UNITS = KC ? ROWS * BK / 8 : ROWS * BK / 32;
     static constexpr int NU = (UNITS + 255) / 256;           // units per thread
     static constexpr int NV = KC ? 1 : 4;                    // 8-value vectors per unit
+    static constexpr int ES = IO == KFH_F32 ? 4 : 2;
     Raw8<IO> v[NU][NV];
-    unsigned bad;                                            // bit i * NV + j: vector j of unit i lies outside
+    const char* base;                                        // of the tile's first row; the same in all lanes
+    long long step, vec;                                     // bytes from a k to the next, from a vector of a unit to the next
+    uint32_t off[NU];                                        // bytes from base of unit i at k = 0
+    unsigned off_rows, bad;                                  // bit i * NV + j: vector j of unit i lies outside (rows only / in all)
 
-    __device__ __forceinline__ void fetch(const void* src, long long ld, long long row0, long long rmax,
-                                          long long k0, long long kmax, int tid) {
-        bad = 0;
+    // k of unit u inside the tile
+    static __device__ __forceinline__ int unit_k(int u) {
+        return KIND == K_MAJOR ? (u % (BK / 8)) * 8 : KIND == K_BLOCK ? (u / ROWS) * 8 : (u % (BK / 4)) * 4;
+    }
+    // what does not change along the contraction: every later address is base + k * step + off + j * vec.
+    // A row behind the last reads the last one's values, which commit clears.
+    __device__ __forceinline__ void init(const void* src, long long ld, long long row0, long long rmax, int tid) {
+        const int left = (int)min(rmax - row0, (long long)ROWS);          // rows of this tile
+        const int nhb = (int)(ld >> 5);
+        off_rows = 0;
+        const char* const s = static_cast<const char*>(src);
+        if constexpr (KIND == K_MAJOR) { base = s + row0 * ld * ES; step = ES; vec = 0; }
+        else if constexpr (KIND == R_MAJOR) { base = s + row0 * ES; step = vec = ld * ES; }
+        else if constexpr (KIND == K_BLOCK) { base = s + (row0 >> 5) * nhb * 2048; step = 64; vec = 0; }   // 32 k: 2 KiB
+        else { base = s + (row0 >> 5) * 2048; step = (long long)nhb * 64; vec = 16; }                       // 32 k: nhb blocks
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int u = i * 256 + tid;
-            if constexpr (KC) {
-                const long long r = row0 + u / (BK / 8), k = k0 + (u % (BK / 8)) * 8;
-                bad |= (unsigned)(r >= rmax || k >= kmax) << i;
-                v[i][0].get(src, (size_t)(min(r, rmax - 1) * ld + min(k, kmax - 8)));
-            } else {
-                const long long r = row0 + (u / (BK / 4)) * 8, k = k0 + (u % (BK / 4)) * 4;
+            const int u = min(i * 256 + tid, UNITS - 1), k = unit_k(u);
+            int r = KIND == K_MAJOR ? u / (BK / 8) : KIND == K_BLOCK ? u % ROWS : (u / (BK / 4)) * 8;
+            if (r >= left) {
+                off_rows |= ((1u << NV) - 1) << (i * NV);
+                r = KC ? left - 1 : left - 8;
+            }
+            if constexpr (KIND == K_MAJOR) off[i] = (uint32_t)(r * (int)ld + k) * ES;
+            else if constexpr (KIND == R_MAJOR) off[i] = (uint32_t)(k * (int)ld + r) * ES;
+            else if constexpr (KIND == K_BLOCK)
+                off[i] = (uint32_t)(((r >> 5) * nhb + (k >> 5)) * 128 + ((k >> 3) & 3) * 32 + (r & 31)) * 16;
+            else
+                off[i] = (uint32_t)(((k >> 5) * nhb + (r >> 5)) * 128 + ((r >> 3) & 3) * 32 + (k & 31)) * 16;
+        }
+    }
+    // the tile at k0 < kmax; only a tile that reaches behind kmax looks at single vectors (they read the
+    // tile's first k instead, which lies inside)
+    __device__ __forceinline__ void fetch(long long k0, long long kmax, int tid) {
+        const char* const b = base + k0 * step;
+        bad = off_rows;
+        if (k0 + BK <= kmax) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    bad |= (unsigned)(r >= rmax || k + j >= kmax) << (4 * i + j);
-                    v[i][j].get(src, (size_t)(min(k + j, kmax - 1) * ld + min(r, rmax - 8)));
+            for (int i = 0; i < NU; ++i)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) v[i][j].get(b + j * vec, off[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const int k = unit_k(min(i * 256 + tid, UNITS - 1));
+                // off of the same row at k = 0
+                uint32_t first = off[i];
+                if constexpr (KIND == K_MAJOR || KIND == R_MAJOR) first -= (uint32_t)(k * step);
+                else if constexpr (KIND == K_BLOCK) first -= (uint32_t)((k >> 5) * 128 + ((k >> 3) & 3) * 32) * 16;
+                else first -= (uint32_t)((k >> 5) * 32 * step) + (k & 31) * 16;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const bool out = k0 + k + j >= kmax;
+                    bad |= (unsigned)out << (i * NV + j);
+                    v[i][j].get(out ? b : b + j * vec, out ? first : off[i]);
                 }
             }
         }
@@ -91,7 +144,12 @@ struct TileLoad {
         for (int i = 0; i < NU; ++i) {
             const int u = i * 256 + tid;
             if (UNITS % 256 != 0 && u >= UNITS) continue;
-            if constexpr (KC) {
+            if constexpr (KIND == K_BLOCK) {
+                const int g = u / ROWS;                      // group 4 b + 2 ks + half: channels 32 b + 16 ks + 4 half + {0..3, 8..11}
+                uint16_t* d = lds + (u % ROWS) * LDK + (g >> 1) * 16 + (g & 1) * 4;
+                *reinterpret_cast<u32x2*>(d) = u32x2{v[i][0].w[0], v[i][0].w[1]};
+                *reinterpret_cast<u32x2*>(d + 8) = u32x2{v[i][0].w[2], v[i][0].w[3]};
+            } else if constexpr (KC) {
                 uint16_t* d = lds + (u / (BK / 8)) * LDK + (u % (BK / 8)) * 8;
                 if constexpr (PARTS == 1) {
                     *reinterpret_cast<u32x4*>(d) = v[i][0].w;
@@ -108,15 +166,17 @@ struct TileLoad {
                     }
                 }
             } else {
-                uint16_t* d = lds + (u / (BK / 4)) * 8 * LDK + (u % (BK / 4)) * 4;
+                const int g = u / (BK / 4);
+                uint16_t* const d0 = lds + (KIND == R_BLOCK ? (g >> 1) * 16 + (g & 1) * 4 : g * 8) * LDK + (u % (BK / 4)) * 4;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
+                    uint16_t* const d = d0 + (KIND == R_BLOCK ? 8 * (e >> 2) + (e & 3) : e) * LDK;
                     if constexpr (PARTS == 1) {
                         // half-word e of the four vectors
                         const uint32_t a = v[i][0].w[e >> 1], b = v[i][1].w[e >> 1], c = v[i][2].w[e >> 1], f = v[i][3].w[e >> 1];
                         const u32x2 w = (e & 1) ? u32x2{(a >> 16) | (b & 0xffff0000u), (c >> 16) | (f & 0xffff0000u)}
                                                 : u32x2{(a & 0xffffu) | (b << 16), (c & 0xffffu) | (f << 16)};
-                        *reinterpret_cast<u32x2*>(d + e * LDK) = w;
+                        *reinterpret_cast<u32x2*>(d) = w;
                     } else {
                         float q[4][3];
 #pragma unroll
@@ -124,7 +184,7 @@ struct TileLoad {
 #pragma unroll
                         for (int p = 0; p < 3; ++p) {
                             u32x2 w = {pack_bf16(q[0][p], q[1][p]), pack_bf16(q[2][p], q[3][p])};
-                            *reinterpret_cast<u32x2*>(d + p * PLANE + e * LDK) = w;
+                            *reinterpret_cast<u32x2*>(d + p * PLANE) = w;
                         }
                     }
                 }
@@ -189,18 +249,20 @@ __device__ __forceinline__ void store4(void* base, size_t e, float a, float b, f
 }
 
 // Workgroups are dealt to the 8 XCDs in turn, each with an L2 of its own: the `nt` tiles that share a
-// row tile follow each other on one XCD, so its rows are read from memory once.  With few row tiles
-// that would leave XCDs idle (one row tile: seven of them), and the tiles are simply counted through.
-constexpr long long kXcdRows = 64;
+// row tile follow each other on one XCD, so its rows are read from memory once (without it the weight
+// gradient 2048 x 256 over 146689 rows took 287 us instead of 198).  With few row tiles, unless they
+// divide evenly, that would leave XCDs idle, and the tiles are simply counted through.
+__host__ __device__ constexpr bool xcd_dealt(long long mtiles) { return mtiles >= 64 || mtiles % 8 == 0; }
 __device__ __forceinline__ bool xcd_tile(long long id, long long mtiles, int nt, long long& mt, int& n) {
-    const long long slot = mtiles >= kXcdRows ? id >> 3 : id;
+    const bool dealt = xcd_dealt(mtiles);
+    const long long slot = dealt ? id >> 3 : id;
     mt = slot / nt;
     n = (int)(slot - mt * nt);
-    if (mtiles >= kXcdRows) mt = mt * 8 + (id & 7);
+    if (dealt) mt = mt * 8 + (id & 7);
     return mt < mtiles;
 }
 static unsigned xcd_grid(long long mtiles, int nt) {
-    return (unsigned)((mtiles >= kXcdRows ? (mtiles + 7) / 8 * 8 : mtiles) * nt);
+    return (unsigned)((xcd_dealt(mtiles) ? (mtiles + 7) / 8 * 8 : mtiles) * nt);
 }
 
 // A finished tile of RM rows x RN columns goes through LDS so that it leaves in whole rows (16 bytes a
@@ -259,23 +321,23 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const void* __restrict_
     const int f0 = ft * 64;
     f32x16 u[NA][1], v[NA][1], g[NA][1];
     zero_acc(u); zero_acc(v); zero_acc(g);
-    TileLoad<IO, true, TM, BK> lx;
-    TileLoad<IO, true, 64, BK> lu, lv;
-    TileLoad<IO, false, 64, BK> lo;
-    lx.fetch(x, C, m0, M, 0, C, tid);
-    lu.fetch(w_in, C, f0, F, 0, C, tid);
-    lv.fetch(w_in, C, (long long)F + f0, 2LL * F, 0, C, tid);
+    TileLoad<IO, K_MAJOR, TM, BK> lx;
+    TileLoad<IO, K_MAJOR, 64, BK> lu, lv;
+    TileLoad<IO, R_MAJOR, 64, BK> lo;
+    lx.init(x, C, m0, M, tid);
+    lu.init(w_in, C, f0, F, tid);
+    lv.init(w_in, C, (long long)F + f0, 2LL * F, tid);
+    lx.fetch(0, C, tid); lu.fetch(0, C, tid); lv.fetch(0, C, tid);
     for (int k0 = 0; k0 < C; k0 += BK) {
         __syncthreads();
         lx.commit(sa, tid); lu.commit(su, tid); lv.commit(sv, tid);
         __syncthreads();
         if (k0 + BK < C) {
-            lx.fetch(x, C, m0, M, k0 + BK, C, tid);
-            lu.fetch(w_in, C, f0, F, k0 + BK, C, tid);
-            lv.fetch(w_in, C, (long long)F + f0, 2LL * F, k0 + BK, C, tid);
+            lx.fetch(k0 + BK, C, tid); lu.fetch(k0 + BK, C, tid); lv.fetch(k0 + BK, C, tid);
         } else if (BWD) {
-            lx.fetch(dy, C, m0, M, 0, C, tid);
-            lo.fetch(w_out, F, f0, F, 0, C, tid);
+            lx.init(dy, C, m0, M, tid);
+            lo.init(w_out, F, f0, F, tid);
+            lx.fetch(0, C, tid); lo.fetch(0, C, tid);
         }
         tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), su, wn * 32, lane, u);
         tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), sv, wn * 32, lane, v);
@@ -286,8 +348,7 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const void* __restrict_
             lx.commit(sa, tid); lo.commit(su, tid);
             __syncthreads();
             if (k0 + BK < C) {
-                lx.fetch(dy, C, m0, M, k0 + BK, C, tid);
-                lo.fetch(w_out, F, f0, F, k0 + BK, C, tid);
+                lx.fetch(k0 + BK, C, tid); lo.fetch(k0 + BK, C, tid);
             }
             tile_mma<IO, NA, 1, TM, 64, BK>(sa, wm * (TM / 2), su, wn * 32, lane, g);
         }
@@ -331,7 +392,7 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const void* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------
-// out[m][n] = sum_k A(m, k) B(n, k); AKC / BKC as TileLoad's KC; a workgroup owns T x T results, a
+// out[m][n] = sum_k A(m, k) B(n, k); AK / BK_ as TileLoad's KIND; a workgroup owns T x T results, a
 // wavefront T/2 x T/2.  The contraction is cut into `splits` ranges of kper; with more than one the
 // results are fp32 partial tiles at out + range * Mo * No (PART), else they are written as IO.
 // ---------------------------------------------------------------------------------------------
@@ -342,7 +403,7 @@ template <int IO, int T> constexpr int gemm_lds(bool part) {
     return in > out ? in : out;
 }
 
-template <int IO, bool AKC, bool BKC, bool PART, int T>
+template <int IO, int AK, int BK_, bool PART, int T>
 __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ A, long long lda,
                                                        const void* __restrict__ B, long long ldb, void* __restrict__ out,
                                                        long long Mo, int No, long long K, long long kper, int splits) {
@@ -371,16 +432,18 @@ __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ 
     const long long kb = z * kper, ke = min(kb + kper, K);
     f32x16 acc[NA][NA];
     zero_acc(acc);
-    TileLoad<IO, AKC, T, BK> la;
-    TileLoad<IO, BKC, T, BK> lb;
+    TileLoad<IO, AK, T, BK> la;
+    TileLoad<IO, BK_, T, BK> lb;
     // two k-tiles ahead: while the matrix cores work on one from LDS, the next is written to the other LDS
     // buffer and the one after travels from memory to registers; one barrier per k-tile
     const long long steps = kb < ke ? (ke - kb + BK - 1) / BK : 0;
     auto fetch = [&](long long s) {
         if (s >= steps) return;
-        la.fetch(A, lda, m0, Mo, kb + s * BK, ke, tid);
-        lb.fetch(B, ldb, n0, No, kb + s * BK, ke, tid);
+        la.fetch(kb + s * BK, ke, tid);
+        lb.fetch(kb + s * BK, ke, tid);
     };
+    la.init(A, lda, m0, Mo, tid);
+    lb.init(B, ldb, n0, No, tid);
     auto commit = [&](long long s) {
         if (s >= steps) return;
         uint16_t* const b = buf + (s & 1) * BUF;
@@ -495,16 +558,14 @@ __global__ __launch_bounds__(256) void ffn_pack_kernel(const uint16_t* __restric
     dst[slot] = u32x4{v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16), v[6] | (v[7] << 16)};
 }
 
-// two fragments of D[hidden][row] values -> row `p` of a row-major tensor: the halves of the wavefront
-// trade 4-channel groups, so that a lane stores 8 consecutive channels (16 bytes)
-__device__ __forceinline__ void store_hidden(uint16_t* row, int half, bool live, const bf16x8& f0, const bf16x8& f1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const u32x4 w = __builtin_bit_cast(u32x4, i ? f1 : f0);
-        const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        if (live) *reinterpret_cast<u32x4*>(row + 16 * i + 8 * half) = u32x4{a[0], b[0], a[1], b[1]};
-    }
+// the two fragments of a block of 32 rows x 32 hidden channels, as they are: 1 KiB per store, past the
+// caches, which hold the weights.  Hidden values of 146689 x 256 x 1024: without any stores 248 us; row by
+// row in 32-byte pieces 462, whole fragments 408, past the caches 352.  Rows behind the last are zeros, for the sums over rows.
+__device__ __forceinline__ void store_hidden(uint16_t* t, size_t slot, bool live, const bf16x8& f0, const bf16x8& f1) {
+    const u32x4 none = {0u, 0u, 0u, 0u};
+    u32x4* const o = reinterpret_cast<u32x4*>(t) + slot;
+    __builtin_nontemporal_store(live ? __builtin_bit_cast(u32x4, f0) : none, o);
+    __builtin_nontemporal_store(live ? __builtin_bit_cast(u32x4, f1) : none, o + 64);
 }
 
 template <int KS, bool BWD, bool FUSE, int NW, int OCC>
@@ -512,13 +573,13 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
                                                                   const uint16_t* __restrict__ dy,
                                                                   const u32x4* __restrict__ wp, uint16_t* __restrict__ h,
                                                                   uint16_t* __restrict__ d, uint16_t* __restrict__ out, long long M,
-                                                                  int F, int steps_per) {
+                                                                  int F) {
     constexpr int C = 16 * KS, NF = stream_frags<KS, BWD, FUSE>(), NT = NW * 64, NB = FUSE ? KS / 2 : 1;
     constexpr int SLOTS = NF * 64, NPRE = (SLOTS + NT - 1) / NT;
     __shared__ __attribute__((aligned(16))) u32x4 smem[2 * SLOTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const long long p0 = (long long)blockIdx.x * (32 * NW) + wave * 32;
-    const int s0 = blockIdx.y * steps_per, s1 = min(s0 + steps_per, F / 32);
+    const int steps = F / 32;
     u32x4 pre[NPRE];
     auto fetch = [&](int s) {
 #pragma unroll
@@ -529,7 +590,7 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
         for (int i = 0; i < NPRE; ++i)
             if (SLOTS % NT == 0 || i * NT + tid < SLOTS) smem[b * SLOTS + i * NT + tid] = pre[i];
     };
-    fetch(s0);
+    fetch(0);
     const long long p = p0 + col;
     const bool live = p < M;
     const size_t row = (size_t)min(p, M - 1) * C + 8 * half;
@@ -549,10 +610,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
 #pragma unroll
             for (int v = 0; v < 16; ++v) oacc[n][v] = 0.f;
     }
-    for (int s = s0; s < s1; ++s) {
-        if (s + 1 < s1) fetch(s + 1);
-        const bf16x8* w = reinterpret_cast<const bf16x8*>(smem + ((s - s0) & 1) * SLOTS) + lane;
-        f32x16 u, v, g;
+    f32x16 u, v, g;
+    auto products = [&](const bf16x8* w) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) { u[i] = 0.f; v[i] = 0.f; g[i] = 0.f; }
 #pragma unroll
@@ -561,7 +620,9 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
             v = mfma32(w[(KS + ks) * 64], xf[ks], v);
             if constexpr (BWD) g = mfma32(w[(2 * KS + ks) * 64], yf[ks], g);
         }
-        const size_t hrow = (size_t)p * F + s * 32;
+    };
+    // activation of step s, its second product (FUSE) and its stores
+    auto finish = [&](int s, const bf16x8* w) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float sg = sigmoidf_fast(u[i]), us = u[i] * sg;
@@ -575,9 +636,9 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
             }
         }
         bf16x8 a0, a1;
+        acc_to_frags(u, a0, a1);
         if constexpr (BWD) {
             bf16x8 b0, b1, h0, h1;
-            acc_to_frags(u, a0, a1);
             acc_to_frags(v, b0, b1);
             acc_to_frags(g, h0, h1);
             if constexpr (FUSE) {
@@ -589,22 +650,27 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
                     oacc[n] = mfma32(b1, w[(4 * KS + 2 * n + 1) * 64], oacc[n]);
                 }
             }
-            store_hidden(h + hrow, half, live, h0, h1);
-            store_hidden(d + 2 * hrow - s * 32, half, live, a0, a1);
-            store_hidden(d + 2 * hrow - s * 32 + F, half, live, b0, b1);
-        } else {
-            acc_to_frags(u, a0, a1);
-            if constexpr (FUSE) {
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    oacc[n] = mfma32(a0, w[(2 * KS + 2 * n) * 64], oacc[n]);
-                    oacc[n] = mfma32(a1, w[(2 * KS + 2 * n + 1) * 64], oacc[n]);
-                }
-            } else {
-                store_hidden(h + hrow, half, live, a0, a1);
+            if (p0 < M) {
+                store_hidden(h, hidden_slot(p, s, F / 32, 0, half), live, h0, h1);
+                store_hidden(d, hidden_slot(p, s, F / 16, 0, half), live, a0, a1);
+                store_hidden(d, hidden_slot(p, F / 32 + s, F / 16, 0, half), live, b0, b1);
             }
+        } else if constexpr (FUSE) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                oacc[n] = mfma32(a0, w[(2 * KS + 2 * n) * 64], oacc[n]);
+                oacc[n] = mfma32(a1, w[(2 * KS + 2 * n + 1) * 64], oacc[n]);
+            }
+        } else {
+            if (p0 < M) store_hidden(h, hidden_slot(p, s, F / 32, 0, half), live, a0, a1);
         }
-        if (s + 1 < s1) commit((s + 1 - s0) & 1);
+    };
+    for (int s = 0; s < steps; ++s) {
+        if (s + 1 < steps) fetch(s + 1);
+        const bf16x8* w = reinterpret_cast<const bf16x8*>(smem + (s & 1) * SLOTS) + lane;
+        products(w);
+        finish(s, w);
+        if (s + 1 < steps) commit((s + 1) & 1);
         __syncthreads();
     }
     if constexpr (FUSE) {
@@ -634,15 +700,16 @@ static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
 // when there are few of them: they are taken when they give every CU a workgroup.
 static bool big_tiles(long long a, long long b, long long more = 1) { return up_div(a, 128) * up_div(b, 128) * more >= 256; }
 
-// Ranges of rows the weight gradients are summed over in parallel: four workgroups per CU, at least
-// 256 rows each.
+// Ranges of rows the weight gradients are summed over in parallel: two workgroups per CU (as many as fit
+// with 128 x 128 tiles; more would only add partial sums), at least 256 rows each.
 struct Wgrad { int T, splits; long long per; };
 static Wgrad wgrad_plan(long long M, long long a, long long b, int io_dtype) {
     Wgrad w;
     const long long most = max(1LL, up_div(M, 256));
     w.T = io_dtype == KFH_BF16 && big_tiles(a, b, most) ? 128 : 64;
     const long long tiles = up_div(a, w.T) * up_div(b, w.T);
-    w.splits = (int)min(min(max(1LL, 1024 / tiles), most), 256LL);
+    w.splits = (int)min(min(max(1LL, 512 / tiles), most), 256LL);
+    if (w.splits > 8) w.splits = w.splits / 8 * 8;           // whole rounds over the XCDs
     w.per = up_div(up_div(M, w.splits), 64) * 64;
     return w;
 }
@@ -675,16 +742,18 @@ static size_t stream_pack_bytes(int C, int F, int backward) {
     return (size_t)(F / 32) * nf * 1024;
 }
 
-// workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F]; packed weights of the
+// workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F], row-major or (streamed) in
+// blocks; packed weights of the
 // streamed kernels; partial sums
 struct FfnWs { size_t h, d, pack, part, total; };
 static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     const size_t e = io_dtype == KFH_F32 ? 4 : 2;
     const bool st = streamed(M, C, F, io_dtype), fused = st && C <= 128;
+    const size_t rows = st ? (size_t)up_div(M, 32) * 32 : (size_t)M;         // whole blocks
     FfnWs w;
     w.h = 0;
-    w.d = w.h + (backward || !fused ? up256((size_t)M * F * e) : 0);
-    w.pack = w.d + (backward ? up256((size_t)M * 2 * F * e) : 0);
+    w.d = w.h + (backward || !fused ? up256(rows * F * e) : 0);
+    w.pack = w.d + (backward ? up256(rows * 2 * F * e) : 0);
     w.part = w.pack + (st ? up256(stream_pack_bytes(C, F, backward)) : 0);
     size_t part = fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype);
     if (backward) part = max(part, wgrad_part_bytes(M, C, F, io_dtype));
@@ -716,48 +785,48 @@ static void hidden(const void* x, const void* dy, const void* w_in, const void* 
                        w_out, h, d, M, C, F);
 }
 
-template <int IO, bool AKC, bool BKC, bool PART, int T>
+template <int IO, int AK, int BK_, bool PART, int T>
 static void gemm(const void* A, long long lda, const void* B, long long ldb, void* out, long long Mo, int No, long long K,
                  long long kper, int splits, hipStream_t stream) {
     const long long mt = up_div(Mo, T), nt = up_div(No, T);
-    hipLaunchKernelGGL((ffn_gemm_kernel<IO, AKC, BKC, PART, T>),
+    hipLaunchKernelGGL((ffn_gemm_kernel<IO, AK, BK_, PART, T>),
                        dim3(PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(256), 0, stream, A, lda, B,
                        ldb, out, Mo, No, K, kper, splits);
 }
 
-// out [Mo, No] = A [Mo, K] times B, [No, K] or (BKC = false) [K, No]; part: product_part_bytes
-template <int IO, bool BKC>
+// out [Mo, No] = A [Mo, K] (AK) times B, [No, K] (K_MAJOR) or [K, No] (R_MAJOR); part: product_part_bytes
+template <int IO, int AK, int BK_>
 static void product(const void* A, long long lda, const void* B, long long ldb, void* out, float* part, long long Mo, int No,
                     long long K, hipStream_t stream) {
     const int splits = product_splits(Mo, No, K, IO);
     if (splits > 1) {
         const long long BK = IO == KFH_F32 ? 32 : 64, per = up_div(up_div(K, BK), splits) * BK;
-        gemm<IO, true, BKC, true, 64>(A, lda, B, ldb, part, Mo, No, K, per, splits, stream);
+        gemm<IO, AK, BK_, true, 64>(A, lda, B, ldb, part, Mo, No, K, per, splits, stream);
         sum_parts(part, splits, Mo * No, out, IO, stream);
         return;
     }
     if constexpr (IO == KFH_BF16) {
         if (big_tiles(Mo, No)) {
-            gemm<IO, true, BKC, false, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
+            gemm<IO, AK, BK_, false, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
             return;
         }
     }
-    gemm<IO, true, BKC, false, 64>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
+    gemm<IO, AK, BK_, false, 64>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
 }
 
-// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]
-template <int IO>
+// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]; AK, BK_: R_MAJOR or R_BLOCK
+template <int IO, int AK, int BK_>
 static void wgrad(const void* A, int Ma, const void* B, int Nb, float* part, void* out, int out_dtype, long long M,
                   hipStream_t stream) {
     const Wgrad w = wgrad_plan(M, Ma, Nb, IO);
     bool done = false;
     if constexpr (IO == KFH_BF16) {
         if (w.T == 128) {
-            gemm<IO, false, false, true, 128>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+            gemm<IO, AK, BK_, true, 128>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
             done = true;
         }
     }
-    if (!done) gemm<IO, false, false, true, 64>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+    if (!done) gemm<IO, AK, BK_, true, 64>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
     sum_parts(part, w.splits, (long long)Ma * Nb, out, out_dtype, stream);
 }
 
@@ -771,15 +840,10 @@ static void stream(const void* x, const void* dy, const void* w_in, const void* 
     const long long slots = (long long)(F / 32) * stream_frags<KS, BWD, FUSE>() * 64;
     hipLaunchKernelGGL((ffn_pack_kernel<KS, BWD, FUSE>), dim3((unsigned)up_div(slots, 256)), dim3(256), 0, stream,
                        static_cast<const uint16_t*>(w_in), static_cast<const uint16_t*>(w_out), pack, F, slots);
-    // without the second product the hidden channels can be dealt out as well: towards eight rounds of
-    // workgroups, so that the last, partly filled one costs little
     const long long tiles = up_div(M, 32 * NW);
-    const int steps = F / 32, parts = FUSE ? 1 : (int)max(1LL, min(2048 / tiles, (long long)steps / 4));
-    const int per = (int)up_div(steps, parts);
-    hipLaunchKernelGGL((ffn_stream_kernel<KS, BWD, FUSE, NW, OCC>), dim3((unsigned)tiles, (unsigned)up_div(steps, per)), dim3(NW * 64),
-                       0, stream, static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(dy), pack,
-                       reinterpret_cast<uint16_t*>(ws + w.h), reinterpret_cast<uint16_t*>(ws + w.d), static_cast<uint16_t*>(out), M, F,
-                       per);
+    hipLaunchKernelGGL((ffn_stream_kernel<KS, BWD, FUSE, NW, OCC>), dim3((unsigned)tiles), dim3(NW * 64), 0, stream,
+                       static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(dy), pack,
+                       reinterpret_cast<uint16_t*>(ws + w.h), reinterpret_cast<uint16_t*>(ws + w.d), static_cast<uint16_t*>(out), M, F);
 }
 template <bool BWD>
 static void stream_by_width(int C, const void* x, const void* dy, const void* w_in, const void* w_out, char* ws,
@@ -796,7 +860,11 @@ static void forward_t(const void* x, const void* w_in, const void* w_out, void* 
     const bool st = streamed(M, C, F, IO);
     if (st) stream_by_width<false>(C, x, nullptr, w_in, w_out, ws, w, y, M, F, stream);
     else hidden<IO, false>(x, nullptr, w_in, nullptr, ws + w.h, nullptr, M, C, F, stream);
-    if (!(st && C <= 128)) product<IO, true>(ws + w.h, F, w_out, F, y, reinterpret_cast<float*>(ws + w.part), M, C, F, stream);
+    float* const part = reinterpret_cast<float*>(ws + w.part);
+    if (!st) product<IO, K_MAJOR, K_MAJOR>(ws + w.h, F, w_out, F, y, part, M, C, F, stream);
+    if constexpr (IO == KFH_BF16) {
+        if (st && C > 128) product<IO, K_BLOCK, K_MAJOR>(ws + w.h, F, w_out, F, y, part, M, C, F, stream);
+    }
 }
 
 template <int IO>
@@ -807,11 +875,19 @@ static void backward_t(const void* dy, const void* x, const void* w_in, const vo
     char* const d = ws + w.d;
     float* const part = reinterpret_cast<float*>(ws + w.part);
     const bool st = streamed(M, C, F, IO);
-    if (st) stream_by_width<true>(C, x, dy, w_in, w_out, ws, w, dx, M, F, stream);
-    else hidden<IO, true>(x, dy, w_in, w_out, h, d, M, C, F, stream);
-    if (dw_out) wgrad<IO>(dy, C, h, F, part, dw_out, dw_dtype, M, stream);
-    if (dw_in) wgrad<IO>(d, 2 * F, x, C, part, dw_in, dw_dtype, M, stream);
-    if (dx && !(st && C <= 128)) product<IO, false>(d, 2LL * F, w_in, C, dx, part, M, C, 2LL * F, stream);
+    if constexpr (IO == KFH_BF16) {
+        if (st) {
+            stream_by_width<true>(C, x, dy, w_in, w_out, ws, w, dx, M, F, stream);
+            if (dw_out) wgrad<IO, R_MAJOR, R_BLOCK>(dy, C, h, F, part, dw_out, dw_dtype, M, stream);
+            if (dw_in) wgrad<IO, R_BLOCK, R_MAJOR>(d, 2 * F, x, C, part, dw_in, dw_dtype, M, stream);
+            if (dx && C > 128) product<IO, K_BLOCK, R_MAJOR>(d, 2LL * F, w_in, C, dx, part, M, C, 2LL * F, stream);
+            return;
+        }
+    }
+    hidden<IO, true>(x, dy, w_in, w_out, h, d, M, C, F, stream);
+    if (dw_out) wgrad<IO, R_MAJOR, R_MAJOR>(dy, C, h, F, part, dw_out, dw_dtype, M, stream);
+    if (dw_in) wgrad<IO, R_MAJOR, R_MAJOR>(d, 2 * F, x, C, part, dw_in, dw_dtype, M, stream);
+    if (dx) product<IO, K_MAJOR, R_MAJOR>(d, 2LL * F, w_in, C, dx, part, M, C, 2LL * F, stream);
 }
 
 void launch_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, void* y, char* ws, long long M,
