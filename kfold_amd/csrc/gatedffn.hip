@@ -57,14 +57,14 @@ __device__ __forceinline__ size_t hidden_slot(long long m, int hb, int nhb, int 
     return ((size_t)((m >> 5) * nhb + hb) * 2 + ks) * 64 + half * 32 + (m & 31);
 }
 
-template <int IO, int KIND, int ROWS, int BK>
+template <int IO, int KIND, int ROWS, int BK, int NT = 256>
 struct TileLoad {
     static constexpr bool KC = KIND == K_MAJOR || KIND == K_BLOCK;
     static constexpr int PARTS = parts_of<IO>();
     static constexpr int LDK = BK + 8;                       // bf16 per stored row
     static constexpr int PLANE = ROWS * LDK;                 // bf16 per part
     static constexpr int UNITS = KC ? ROWS * BK / 8 : ROWS * BK / 32;
-    static constexpr int NU = (UNITS + 255) / 256;           // units per thread
+    static constexpr int NU = (UNITS + NT - 1) / NT;           // units per thread
     static constexpr int NV = KC ? 1 : 4;                    // 8-value vectors per unit
     static constexpr int ES = IO == KFH_F32 ? 4 : 2;
     Raw8<IO> v[NU][NV];
@@ -90,7 +90,7 @@ struct TileLoad {
         else { base = s + (row0 >> 5) * 2048; step = (long long)nhb * 64; vec = 16; }                       // 32 k: nhb blocks
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int u = min(i * 256 + tid, UNITS - 1), k = unit_k(u);
+            const int u = min(i * NT + tid, UNITS - 1), k = unit_k(u);
             int r = KIND == K_MAJOR ? u / (BK / 8) : KIND == K_BLOCK ? u % ROWS : (u / (BK / 4)) * 8;
             if (r >= left) {
                 off_rows |= ((1u << NV) - 1) << (i * NV);
@@ -117,7 +117,7 @@ struct TileLoad {
         } else {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
-                const int k = unit_k(min(i * 256 + tid, UNITS - 1));
+                const int k = unit_k(min(i * NT + tid, UNITS - 1));
                 // off of the same row at k = 0
                 uint32_t first = off[i];
                 if constexpr (KIND == K_MAJOR || KIND == R_MAJOR) first -= (uint32_t)(k * step);
@@ -142,8 +142,8 @@ struct TileLoad {
         }
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int u = i * 256 + tid;
-            if (UNITS % 256 != 0 && u >= UNITS) continue;
+            const int u = i * NT + tid;
+            if (UNITS % NT != 0 && u >= UNITS) continue;
             if constexpr (KIND == K_BLOCK) {
                 const int g = u / ROWS;                      // group 4 b + 2 ks + half: channels 32 b + 16 ks + 4 half + {0..3, 8..11}
                 uint16_t* d = lds + (u % ROWS) * LDK + (g >> 1) * 16 + (g & 1) * 4;
@@ -267,7 +267,7 @@ static unsigned xcd_grid(long long mtiles, int nt) {
 
 // A finished tile of RM rows x RN columns goes through LDS so that it leaves in whole rows (16 bytes a
 // lane, 2 RN bytes a row) instead of 8 bytes of 64 different rows.  put: four consecutive columns.
-template <int IO, int RM, int RN>
+template <int IO, int RM, int RN, int NT = 256>
 struct TileStore {
     static constexpr int ES = IO == KFH_F32 ? 4 : 2;
     static constexpr int LD = RN * ES + 16;                  // bytes per staged row
@@ -279,8 +279,8 @@ struct TileStore {
                                                  int N, int tid) {
         constexpr int PER = RN * ES / 16;                    // 16-byte pieces per row
 #pragma unroll
-        for (int i = 0; i < RM * PER / 256; ++i) {
-            const int u = i * 256 + tid, r = u / PER, c = (u % PER) * (16 / ES);
+        for (int i = 0; i < RM * PER / NT; ++i) {
+            const int u = i * NT + tid, r = u / PER, c = (u % PER) * (16 / ES);
             if (m0 + r < M && n0 + c < N)
                 *reinterpret_cast<u32x4*>(static_cast<char*>(out) + ((size_t)(m0 + r) * ld + n0 + c) * ES) =
                     *reinterpret_cast<const u32x4*>(t + r * LD + c * ES);
@@ -392,29 +392,42 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const void* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------
-// out[m][n] = sum_k A(m, k) B(n, k); AK / BK_ as TileLoad's KIND; a workgroup owns T x T results, a
-// wavefront T/2 x T/2.  The contraction is cut into `splits` ranges of kper; with more than one the
-// results are fp32 partial tiles at out + range * Mo * No (PART), else they are written as IO.
+// out[m][n] = sum_k A(m, k) B(n, k); AK / BK_ as TileLoad's KIND; a workgroup of NW wavefronts owns
+// TM x TN results, wavefront (wm, wn) TM / WM x TN / WN of them.  The contraction is cut into `splits`
+// ranges of kper; with more than one the results are fp32 partial tiles at out + range * Mo * No (PART),
+// else they are written as IO.
+//
+// What bounds it is the way of the operands into LDS: with 128 x 128 tiles the weight gradient 2048 x 256
+// over 146689 rows takes 261 us for the loads alone, 100 us for the products alone (1.5 PF/s) and 265 us
+// together.  A 256 x 256 tile asks for half the bytes.
 // ---------------------------------------------------------------------------------------------
-template <int IO, int T> constexpr int gemm_lds(bool part) {
-    constexpr int BK = IO == KFH_F32 ? 32 : 64;
-    const int in = 2 * parts_of<IO>() * 2 * T * (BK + 8) * 2;
-    const int out = part ? TileStore<KFH_F32, T, T / 2>::BYTES : TileStore<IO, T, T / 2>::BYTES;
-    return in > out ? in : out;
-}
+template <int V> struct Int { static constexpr int v = V; };
+template <int TM, int TN> struct Waves {                     // wavefronts of a tile and their arrangement
+    static constexpr int NW = TM * TN >= 256 * 128 ? 8 : 4;
+    static constexpr int WM = NW == 4 || TM < TN || TM == TN ? 2 : 4, WN = NW / WM;
+};
+template <int IO, int TM, int TN, bool PART> struct GemmLds {
+    static constexpr int BK = IO == KFH_F32 ? 32 : 64, NT = Waves<TM, TN>::NW * 64;
+    using Out = TileStore<PART ? (int)KFH_F32 : IO, TM, TN / Waves<TM, TN>::WN, NT>;      // one column of wavefronts
+    static constexpr int IN = 2 * parts_of<IO>() * (TM + TN) * (BK + 8) * 2;
+    static constexpr int BYTES = IN > Out::BYTES ? IN : Out::BYTES;
+};
 
-template <int IO, int AK, int BK_, bool PART, int T>
-__global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ A, long long lda,
-                                                       const void* __restrict__ B, long long ldb, void* __restrict__ out,
-                                                       long long Mo, int No, long long K, long long kper, int splits) {
-    constexpr int BK = IO == KFH_F32 ? 32 : 64, LDK = BK + 8, P = parts_of<IO>(), NA = T / 64;
-    __shared__ __attribute__((aligned(16))) char smem[gemm_lds<IO, T>(PART)];
-    constexpr int BUF = 2 * P * T * LDK;
+template <int IO, int AK, int BK_, bool PART, int TM, int TN>
+__global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
+    const void* __restrict__ A, long long lda, const void* __restrict__ B, long long ldb, void* __restrict__ out,
+    long long Mo, int No, long long K, long long kper, int splits) {
+    using W = Waves<TM, TN>;
+    using Lds = GemmLds<IO, TM, TN, PART>;
+    constexpr int BK = Lds::BK, LDK = BK + 8, P = parts_of<IO>(), NT = Lds::NT;
+    constexpr int RM = TM / W::WM, RN = TN / W::WN, NA = RM / 32, NB = RN / 32;
+    __shared__ __attribute__((aligned(16))) char smem[Lds::BYTES];
+    constexpr int BUF = P * (TM + TN) * LDK;
     uint16_t* const buf = reinterpret_cast<uint16_t*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave & 1, wn = wave >> 1;
-    const long long mtiles = (Mo + T - 1) / T;
-    const int ntiles = (No + T - 1) / T;
+    const int wm = wave % W::WM, wn = wave / W::WM;
+    const long long mtiles = (Mo + TM - 1) / TM;
+    const int ntiles = (No + TN - 1) / TN;
     // tiles that share operand rows follow each other on one XCD: those of a row tile, or (PART) all
     // tiles of one range of the contraction
     long long mt, z = 0;
@@ -427,13 +440,13 @@ __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ 
     } else {
         if (!xcd_tile(blockIdx.x, mtiles, ntiles, mt, nt)) return;
     }
-    const long long m0 = mt * T;
-    const int n0 = nt * T;
+    const long long m0 = mt * TM;
+    const int n0 = nt * TN;
     const long long kb = z * kper, ke = min(kb + kper, K);
-    f32x16 acc[NA][NA];
+    f32x16 acc[NA][NB];
     zero_acc(acc);
-    TileLoad<IO, AK, T, BK> la;
-    TileLoad<IO, BK_, T, BK> lb;
+    TileLoad<IO, AK, TM, BK, NT> la;
+    TileLoad<IO, BK_, TN, BK, NT> lb;
     // two k-tiles ahead: while the matrix cores work on one from LDS, the next is written to the other LDS
     // buffer and the one after travels from memory to registers; one barrier per k-tile
     const long long steps = kb < ke ? (ke - kb + BK - 1) / BK : 0;
@@ -448,7 +461,7 @@ __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ 
         if (s >= steps) return;
         uint16_t* const b = buf + (s & 1) * BUF;
         la.commit(b, tid);
-        lb.commit(b + P * T * LDK, tid);
+        lb.commit(b + P * TM * LDK, tid);
     };
     fetch(0);
     commit(0);
@@ -458,28 +471,27 @@ __global__ __launch_bounds__(256) void ffn_gemm_kernel(const void* __restrict__ 
         commit(s + 1);
         fetch(s + 2);
         const uint16_t* const b = buf + (s & 1) * BUF;
-        tile_mma<IO, NA, NA, T, T, BK>(b, wm * (T / 2), b + P * T * LDK, wn * (T / 2), lane, acc);
+        tile_mma<IO, NA, NB, TM, TN, BK>(b, wm * RM, b + P * TM * LDK, wn * RN, lane, acc);
         __syncthreads();
     }
-    // through LDS in two halves of T / 2 columns
-    constexpr int OIO = PART ? KFH_F32 : IO;
-    using Out = TileStore<OIO, T, T / 2>;
+    // through LDS, one column of wavefronts at a time
+    using Out = typename Lds::Out;
     char* const base = static_cast<char*>(out) + (PART ? (size_t)z * Mo * No * 4 : 0);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (half) __syncthreads();
-        if (wn == half) {
+#pragma unroll 1
+    for (int c = 0; c < W::WN; ++c) {
+        if (c) __syncthreads();
+        if (wn == c) {
 #pragma unroll
             for (int a = 0; a < NA; ++a)
 #pragma unroll
-                for (int b = 0; b < NA; ++b)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        Out::put(smem, wm * (T / 2) + 32 * a + (lane & 31), 32 * b + 8 * q + 4 * (lane >> 5), acc[a][b][4 * q],
+                        Out::put(smem, wm * RM + 32 * a + (lane & 31), 32 * b + 8 * q + 4 * (lane >> 5), acc[a][b][4 * q],
                                  acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]);
         }
         __syncthreads();
-        Out::flush(smem, base, No, m0, Mo, n0 + half * (T / 2), No, tid);
+        Out::flush(smem, base, No, m0, Mo, n0 + c * RN, No, tid);
     }
 }
 
@@ -696,19 +708,28 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 static long long up_div(long long a, long long b) { return (a + b - 1) / b; }
 
-// Tiles of 128 x 128 feed the matrix cores twice as well as tiles of 64 x 64 but leave the chip empty
-// when there are few of them: they are taken when they give every CU a workgroup.
-static bool big_tiles(long long a, long long b, long long more = 1) { return up_div(a, 128) * up_div(b, 128) * more >= 256; }
+// Tile of a product [a, b]: the larger, the fewer bytes per result come into LDS; 256 along a side that has
+// 256, 128 else, as long as every CU gets a workgroup (`more`: ranges the contraction may be cut into), or
+// 64 x 64.  fp32 stays with 64 x 64: its operands take three times the LDS.
+struct Tile { int m, n; };
+static Tile pick_tile(long long a, long long b, long long more, int io_dtype) {
+    if (io_dtype != KFH_BF16) return {64, 64};
+    auto full = [&](int m, int n) { return up_div(a, m) * up_div(b, n) * more >= 256; };
+    const int m = a >= 256 ? 256 : 128, n = b >= 256 ? 256 : 128;
+    if (full(m, n)) return {m, n};
+    if (full(128, 128)) return {128, 128};
+    return {64, 64};
+}
 
-// Ranges of rows the weight gradients are summed over in parallel: two workgroups per CU (as many as fit
-// with 128 x 128 tiles; more would only add partial sums), at least 256 rows each.
-struct Wgrad { int T, splits; long long per; };
+// Ranges of rows the weight gradients are summed over in parallel: one workgroup per CU with large tiles (as
+// many as fit; more would only add partial sums), two with 64 x 64, at least 256 rows each.
+struct Wgrad { Tile t; int splits; long long per; };
 static Wgrad wgrad_plan(long long M, long long a, long long b, int io_dtype) {
     Wgrad w;
     const long long most = max(1LL, up_div(M, 256));
-    w.T = io_dtype == KFH_BF16 && big_tiles(a, b, most) ? 128 : 64;
-    const long long tiles = up_div(a, w.T) * up_div(b, w.T);
-    w.splits = (int)min(min(max(1LL, 512 / tiles), most), 256LL);
+    w.t = pick_tile(a, b, most, io_dtype);
+    const long long tiles = up_div(a, w.t.m) * up_div(b, w.t.n);
+    w.splits = (int)min(min(max(1LL, (w.t.m * w.t.n > 128 * 128 ? 256 : 512) / tiles), most), 256LL);
     if (w.splits > 8) w.splits = w.splits / 8 * 8;           // whole rounds over the XCDs
     w.per = up_div(up_div(M, w.splits), 64) * 64;
     return w;
@@ -769,7 +790,6 @@ static void sum_parts(const float* part, int parts, long long n, void* out, int 
                        out_dtype);
 }
 
-// (fp32 stays with the small tiles: its operands take three times the LDS)
 template <int IO, bool BWD>
 static void hidden(const void* x, const void* dy, const void* w_in, const void* w_out, void* h, void* d, long long M, int C,
                    int F, hipStream_t stream) {
@@ -785,13 +805,13 @@ static void hidden(const void* x, const void* dy, const void* w_in, const void* 
                        w_out, h, d, M, C, F);
 }
 
-template <int IO, int AK, int BK_, bool PART, int T>
+template <int IO, int AK, int BK_, bool PART, int TM, int TN>
 static void gemm(const void* A, long long lda, const void* B, long long ldb, void* out, long long Mo, int No, long long K,
                  long long kper, int splits, hipStream_t stream) {
-    const long long mt = up_div(Mo, T), nt = up_div(No, T);
-    hipLaunchKernelGGL((ffn_gemm_kernel<IO, AK, BK_, PART, T>),
-                       dim3(PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(256), 0, stream, A, lda, B,
-                       ldb, out, Mo, No, K, kper, splits);
+    const long long mt = up_div(Mo, TM), nt = up_div(No, TN);
+    hipLaunchKernelGGL((ffn_gemm_kernel<IO, AK, BK_, PART, TM, TN>),
+                       dim3(PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(Waves<TM, TN>::NW * 64), 0,
+                       stream, A, lda, B, ldb, out, Mo, No, K, kper, splits);
 }
 
 // out [Mo, No] = A [Mo, K] (AK) times B, [No, K] (K_MAJOR) or [K, No] (R_MAJOR); part: product_part_bytes
@@ -801,17 +821,17 @@ static void product(const void* A, long long lda, const void* B, long long ldb, 
     const int splits = product_splits(Mo, No, K, IO);
     if (splits > 1) {
         const long long BK = IO == KFH_F32 ? 32 : 64, per = up_div(up_div(K, BK), splits) * BK;
-        gemm<IO, AK, BK_, true, 64>(A, lda, B, ldb, part, Mo, No, K, per, splits, stream);
+        if constexpr (AK == K_MAJOR) gemm<IO, AK, BK_, true, 64, 64>(A, lda, B, ldb, part, Mo, No, K, per, splits, stream);
         sum_parts(part, splits, Mo * No, out, IO, stream);
         return;
     }
+    const Tile t = pick_tile(Mo, No, 1, IO);
     if constexpr (IO == KFH_BF16) {
-        if (big_tiles(Mo, No)) {
-            gemm<IO, AK, BK_, false, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
-            return;
-        }
+        if (t.n == 256) { gemm<IO, AK, BK_, false, 256, 256>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream); return; }
+        if (t.m == 256) { gemm<IO, AK, BK_, false, 256, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream); return; }
+        if (t.m == 128) { gemm<IO, AK, BK_, false, 128, 128>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream); return; }
     }
-    gemm<IO, AK, BK_, false, 64>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
+    if constexpr (AK == K_MAJOR) gemm<IO, AK, BK_, false, 64, 64>(A, lda, B, ldb, out, Mo, No, K, K, 1, stream);
 }
 
 // out [Ma, Nb] = A [M, Ma]^T B [M, Nb]; AK, BK_: R_MAJOR or R_BLOCK
@@ -819,14 +839,19 @@ template <int IO, int AK, int BK_>
 static void wgrad(const void* A, int Ma, const void* B, int Nb, float* part, void* out, int out_dtype, long long M,
                   hipStream_t stream) {
     const Wgrad w = wgrad_plan(M, Ma, Nb, IO);
+    auto run = [&](auto tm, auto tn) {
+        gemm<IO, AK, BK_, true, decltype(tm)::v, decltype(tn)::v>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+    };
     bool done = false;
     if constexpr (IO == KFH_BF16) {
-        if (w.T == 128) {
-            gemm<IO, AK, BK_, true, 128>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
-            done = true;
-        }
+        done = true;
+        if (w.t.m == 256 && w.t.n == 256) run(Int<256>{}, Int<256>{});
+        else if (w.t.m == 256) run(Int<256>{}, Int<128>{});
+        else if (w.t.n == 256) run(Int<128>{}, Int<256>{});
+        else if (w.t.m == 128) run(Int<128>{}, Int<128>{});
+        else done = false;
     }
-    if (!done) gemm<IO, AK, BK_, true, 64>(A, Ma, B, Nb, part, Ma, Nb, M, w.per, w.splits, stream);
+    if (!done) run(Int<64>{}, Int<64>{});
     sum_parts(part, w.splits, (long long)Ma * Nb, out, out_dtype, stream);
 }
 
