@@ -43,10 +43,10 @@ __global__ __launch_bounds__(256) void ffn_split_kernel(SplitArgs p) {
 // Operands and results in P parts, consecutive planes.  The next D k-tiles travel from memory while the
 // matrix cores work on the present one.
 // ---------------------------------------------------------------------------------------------
-template <int P, int TM> constexpr int hidden_lds(bool bwd) {
+template <int P, int TM> constexpr int hidden_lds() {
     constexpr int BK = P == 3 ? 32 : 64;
     const int in = P * (TM + 128) * (BK + 8) * 2;
-    const int out = P * (bwd ? 3 : 1) * TileStore<KFH_BF16, TM, 64, 256>::BYTES;
+    const int out = P * TileStore<KFH_BF16, TM, 64, 256>::BYTES;
     return in > out ? in : out;
 }
 
@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const uint16_t* __restr
                                                          const uint16_t* __restrict__ w_in,
                                                          const uint16_t* __restrict__ w_out, uint16_t* __restrict__ h,
                                                          uint16_t* __restrict__ d, long long M, int C, int F) {
-    constexpr int BK = P == 3 ? 32 : 64, LDK = BK + 8, NA = TM / 64, D = TM == 64 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) char smem[hidden_lds<P, TM>(BWD)];
+    constexpr int BK = P == 3 ? 32 : 64, LDK = BK + 8, NA = TM / 64, D = P == 1 && TM == 64 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) char smem[hidden_lds<P, TM>()];
     uint16_t* const sa = reinterpret_cast<uint16_t*>(smem);
     uint16_t* const su = sa + P * TM * LDK;
     uint16_t* const sv = su + P * 64 * LDK;
@@ -134,53 +134,51 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const uint16_t* __restr
             }
         }
     }
-    __syncthreads();
-    using Out = TileStore<KFH_BF16, TM, 64, 256>;
-    auto put = [&](int tensor, int r, int f, const float (&o)[4]) {
-        if constexpr (P == 1) {
-            Out::put(smem + tensor * Out::BYTES, r, f, o[0], o[1], o[2], o[3]);
-        } else {
-            float q[4][3];
+    // h, du and dv in the places of dh, u and v (forward: h in the place of u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split3(o[e], q[e]);
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
-            for (int k = 0; k < 3; ++k) Out::put(smem + (tensor * 3 + k) * Out::BYTES, r, f, q[0][k], q[1][k], q[2][k], q[3][k]);
-        }
-    };
-#pragma unroll
-    for (int a = 0; a < NA; ++a) {
-        const int r = wm * (TM / 2) + 32 * a + (lane & 31);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int f = wn * 32 + 8 * q + 4 * (lane >> 5);
-            float hh[4], du[4], dv[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float uu = u[a][0][4 * q + e], vv = v[a][0][4 * q + e];
-                const float s = sigmoidf_fast(uu), us = uu * s;
-                hh[e] = us * vv;
-                if constexpr (BWD) {
-                    const float gg = g[a][0][4 * q + e];
-                    dv[e] = gg * us;
-                    du[e] = gg * vv * (s + us * (1.f - s));
-                }
-            }
-            put(0, r, f, hh);
+        for (int e = 0; e < 16; ++e) {
+            const float uu = u[a][0][e], vv = v[a][0][e];
+            const float s = sigmoidf_fast(uu), us = uu * s;
             if constexpr (BWD) {
-                put(1, r, f, du);
-                put(2, r, f, dv);
+                const float gg = g[a][0][e];
+                g[a][0][e] = us * vv;
+                u[a][0][e] = gg * vv * (s + us * (1.f - s));
+                v[a][0][e] = gg * us;
+            } else {
+                u[a][0][e] = us * vv;
             }
         }
-    }
-    __syncthreads();
+    using Out = TileStore<KFH_BF16, TM, 64, 256>;
+    auto write = [&](const f32x16(&t)[NA][1], uint16_t* dst, long long ld) {      // planes M * ld apart
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-        Out::flush(smem + k * Out::BYTES, h + (size_t)k * M * F, F, m0, M, f0, F, tid);
-        if constexpr (BWD) {
-            uint16_t* const dk = d + (size_t)k * M * 2 * F;
-            Out::flush(smem + (P + k) * Out::BYTES, dk, 2LL * F, m0, M, f0, F, tid);
-            Out::flush(smem + (2 * P + k) * Out::BYTES, dk + F, 2LL * F, m0, M, f0, F, tid);
+        for (int a = 0; a < NA; ++a) {
+            const int r = wm * (TM / 2) + 32 * a + (lane & 31);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int f = wn * 32 + 8 * q + 4 * (lane >> 5);
+                float s[4][3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[e][0] = t[a][0][4 * q + e];
+                    if constexpr (P == 3) split3(t[a][0][4 * q + e], s[e]);
+                }
+#pragma unroll
+                for (int k = 0; k < P; ++k) Out::put(smem + k * Out::BYTES, r, f, s[0][k], s[1][k], s[2][k], s[3][k]);
+            }
         }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < P; ++k) Out::flush(smem + k * Out::BYTES, dst + (size_t)k * M * ld, ld, m0, M, f0, F, tid);
+    };
+    if constexpr (BWD) {
+        write(g, h, F);
+        write(u, d, 2LL * F);
+        write(v, d + F, 2LL * F);
+    } else {
+        write(u, h, F);
     }
 }
 
@@ -307,6 +305,73 @@ __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// The two products of a forward call in bf16 with few rows, where nothing but latency counts: a workgroup
+// owns 32 x 32 results, its wavefronts take the k-steps in turn and read their fragments straight from memory
+// (every load of a batch independent of the others), and the partial sums meet in LDS.
+//   GATED: out[m][n] = silu(A W_n) * (A W_{N+n});  else out[m][n] = A W_n;   A [M, K], W [N or 2N, K]
+// ---------------------------------------------------------------------------------------------
+constexpr int kSmallWaves = 4, kSmallBatch = 4;
+
+template <bool GATED>
+__global__ __launch_bounds__(64 * kSmallWaves) void ffn_small_kernel(const uint16_t* __restrict__ A,
+                                                                     const uint16_t* __restrict__ W,
+                                                                     uint16_t* __restrict__ out, long long M, int N, int K) {
+    constexpr int NB = GATED ? 2 : 1;
+    __shared__ float red[kSmallWaves][NB][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+    const long long m0 = (long long)blockIdx.y * 32;
+    const int n0 = blockIdx.x * 32;
+    const uint16_t* const a = A + (size_t)min(m0 + col, M - 1) * K;
+    const uint16_t* const b = W + (size_t)min(n0 + col, N - 1) * K;
+    f32x16 acc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[j][v] = 0.f;
+    const int steps = (K + 15) / 16;
+    for (int s = wave; s < steps; s += kSmallWaves * kSmallBatch) {
+        u32x4 fa[kSmallBatch], fb[kSmallBatch][NB];
+#pragma unroll
+        for (int i = 0; i < kSmallBatch; ++i) {
+            const int k = min((s + i * kSmallWaves) * 16 + 8 * half, K - 8);
+            fa[i] = *reinterpret_cast<const u32x4*>(a + k);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[i][j] = *reinterpret_cast<const u32x4*>(b + (size_t)j * N * K + k);
+        }
+#pragma unroll
+        for (int i = 0; i < kSmallBatch; ++i) {
+            // a k-step (or its upper half) behind the end: A's values count as zeros
+            const bool in = (s + i * kSmallWaves) * 16 + 8 * half < K;
+            const bf16x8 x = __builtin_bit_cast(bf16x8, in ? fa[i] : u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+                acc[j] = mfma32(__builtin_bit_cast(bf16x8, in ? fb[i][j] : u32x4{0u, 0u, 0u, 0u}), x, acc[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) red[wave][j][v][lane] = acc[j][v];
+    __syncthreads();
+    // wavefront q finishes accumulator rows 4q .. 4q + 3: four consecutive columns of one row per lane
+    float o[NB][4];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[j][e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kSmallWaves; ++w) o[j][e] += red[w][j][4 * wave + e][lane];
+        }
+    if constexpr (GATED) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][e] = o[0][e] * sigmoidf_fast(o[0][e]) * o[1][e];
+    }
+    const int n = n0 + 8 * wave + 4 * half;
+    if (m0 + col < M && n < N) store4<KFH_BF16>(out, (size_t)(m0 + col) * N + n, o[0][0], o[0][1], o[0][2], o[0][3]);
+}
+
 // out[i] = sum of `parts` fp32 values part[z * n + i]: 64 lanes x 4 values per workgroup, its four
 // wavefronts take every fourth part; a fixed order
 __global__ __launch_bounds__(256) void ffn_sum_parts_kernel(const float* __restrict__ part, int parts, long long n,
@@ -387,6 +452,10 @@ static size_t product_part_bytes(long long Mo, long long No, long long K, int io
 static bool streamed(long long M, int C, int F, int io_dtype) {
     return io_dtype == KFH_BF16 && (C == 64 || C == 128 || C == 256) && F % 32 == 0 && M >= 16384;
 }
+
+// Few rows: with fewer than 128 tiles of 64 x 64 hidden values the kernels that work straight from memory are
+// faster (37 x 384 x 768: 10.8 against 14.8 us; 666 rows, 132 tiles: equal; 1000 rows: 20.4 against 13.6).
+static bool few_rows(long long M, int F) { return up_div(M, 64) * up_div(F, 64) < 128; }
 
 // Workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F], row-major in P planes or (streamed)
 // in blocks; packed weights of the streamed kernels; planes of x, w_in, w_out and dy (fp32); partial sums
@@ -524,6 +593,17 @@ static void forward_t(const void* x, const void* w_in, const void* w_out, void* 
         launch_ffn_stream(x, nullptr, w_in, w_out, ws + w.pack, ws + w.h, nullptr, y, M, C, F, stream);
         if (C > 128) product<1, K_BLOCK, K_MAJOR>({ws + w.h, F, 0}, {w_out, F, 0}, y, part, M, C, F, stream);
         return;
+    }
+    if constexpr (P == 1) {
+        if (few_rows(M, F)) {
+            const uint16_t* const xs = static_cast<const uint16_t*>(x);
+            uint16_t* const h = reinterpret_cast<uint16_t*>(ws + w.h);
+            hipLaunchKernelGGL(ffn_small_kernel<true>, dim3((unsigned)up_div(F, 32), (unsigned)up_div(M, 32)), dim3(64 * kSmallWaves), 0,
+                               stream, xs, static_cast<const uint16_t*>(w_in), h, M, F, C);
+            hipLaunchKernelGGL(ffn_small_kernel<false>, dim3((unsigned)up_div(C, 32), (unsigned)up_div(M, 32)), dim3(64 * kSmallWaves), 0,
+                               stream, h, static_cast<const uint16_t*>(w_out), static_cast<uint16_t*>(y), M, C, F);
+            return;
+        }
     }
     hidden<P, false>(x, nullptr, w_in, nullptr, ws + w.h, nullptr, M, C, F, stream);
     product<P, K_MAJOR, K_MAJOR>({ws + w.h, F, M * F * 2}, {w_out, F, 2LL * F * C}, y, part, M, C, F, stream);

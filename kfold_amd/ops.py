@@ -6,6 +6,8 @@ computation happens inside libkfold_hip.so.  All functions require CUDA (ROCm) t
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -573,6 +575,25 @@ def cross_apb_forward(a_q: torch.Tensor, a_k: torch.Tensor, s_q, s_k, pair_bias:
 # ---------------------------------------------------------------------------------------
 # training operators: layer norm, gated feed-forward block, dropout
 # ---------------------------------------------------------------------------------------
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # without the Stream object around it
+
+
+def _stream_of(device: torch.device) -> int:
+    if _raw_stream is not None and device.type == "cuda":
+        return _raw_stream(device.index)
+    return _stream(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """``torch.cuda.device(device)``, or nothing where it is the current device already."""
+    if device.type == "cuda" and torch.cuda.current_device() == device.index:
+        return _HERE
+    return torch.cuda.device(device)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t contiguous and at a 16-byte boundary (a view into a larger tensor may start anywhere)."""
     t = t.contiguous()
@@ -594,6 +615,8 @@ def _affine_f32(w: torch.Tensor | None, C: int, name: str) -> torch.Tensor | Non
         return None
     if w.shape != (C,):
         raise ValueError(f"layer norm: {name} has shape {tuple(w.shape)}, the rows have {C} channels")
+    if w.dtype == torch.float32 and w.is_contiguous():
+        return w
     return w.detach().to(dtype=torch.float32).contiguous()
 
 
@@ -618,9 +641,9 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
         mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
         rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if rows:
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(_lib.lib().kfh_layer_norm_forward(xc.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(mean),
-                                                    _ptr(rstd), rows, C, float(eps), io, _stream(dev)))
+                                                    _ptr(rstd), rows, C, float(eps), io, _stream_of(dev)))
     return (y, mean, rstd) if stats else y
 
 
@@ -650,10 +673,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         ws_bytes = L.kfh_layer_norm_backward_workspace_bytes(rows, C)
         ws = _workspace(workspace, ws_bytes, dev)
     if dx is not None or dw is not None:
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(L.kfh_layer_norm_backward(dyc.data_ptr(), xc.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(w),
                                             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws_bytes, rows, C, io,
-                                            _stream(dev)))
+                                            _stream_of(dev)))
     return dx, dw, db
 
 
@@ -689,9 +712,9 @@ def gated_ffn_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, 
     L = _lib.lib()
     ws_bytes = L.kfh_gated_ffn_workspace_bytes(rows, C, F, 0, io)
     ws = _workspace(workspace, ws_bytes, dev) if ws_bytes else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(L.kfh_gated_ffn_forward(xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), y.data_ptr(), _ptr(ws), ws_bytes,
-                                      rows, C, F, io, _stream(dev)))
+                                      rows, C, F, io, _stream_of(dev)))
     return y
 
 
@@ -720,10 +743,10 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_
     L = _lib.lib()
     ws_bytes = L.kfh_gated_ffn_workspace_bytes(rows, C, F, 1, io)
     ws = _workspace(workspace, ws_bytes, dev) if rows else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(L.kfh_gated_ffn_backward(dyc.data_ptr(), xc.data_ptr(), wi.data_ptr(), wo.data_ptr(), _ptr(dx), _ptr(dwi),
                                        _ptr(dwo), _IO_DTYPES[dw_dtype], _ptr(ws), ws_bytes, rows, C, F, io,
-                                       _stream(dev)))
+                                       _stream_of(dev)))
     return dx, dwi, dwo
 
 
@@ -757,9 +780,9 @@ def _drop(x, residual, p, seed, offset, shared_dim, out):
     y = _result(out, xc, "out")
     if x.numel() == 0:
         return y
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(_lib.lib().kfh_dropout(xc.data_ptr(), _ptr(rc), y.data_ptr(), outer, shared, inner, float(p), seed_ptr,
-                                     seed_val, int(offset) & 0xFFFFFFFFFFFFFFFF, io, _stream(dev)))
+                                     seed_val, int(offset) & 0xFFFFFFFFFFFFFFFF, io, _stream_of(dev)))
     return y
 
 

@@ -298,9 +298,10 @@ def test_gated_ffn_many_rows():
     assert dwi.dtype == F32 and dwo.dtype == F32
     for got, name in ((dx, "dx"), (dwi, "dw_in"), (dwo, "dw_out")):
         within(got, r[name], e[name], name)
-    # rows are independent: the rows of a shorter call are the same bits
+    # a shorter call on the same rows may go through another kernel, which adds in another order: both are
+    # within the bound e of the exact y, so |a - b| <= |a - y| + |b - y| <= 2 e
     part = ops.gated_ffn_forward(xd[:900], wi, wo)
-    assert torch.equal(part, ops.gated_ffn_forward(xd, wi, wo)[:900])
+    within(part, ops.gated_ffn_forward(xd, wi, wo)[:900].cpu(), 2 * e["y"][:900], "y of the first 900 rows")
 
 
 def test_gated_ffn_leaves_what_is_not_its_own():
