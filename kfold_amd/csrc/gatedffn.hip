@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const uint16_t* __restr
 // out[m][n] = sum_k A(m, k) B(n, k), operands in P parts (planes `ap`, `bp` bytes apart); AK / BK_ as
 // TileLoad's KIND; a workgroup of NW wavefronts owns TM x TN results, wavefront (wm, wn) TM / WM x TN / WN
 // of them.  The contraction is cut into `splits` ranges of kper; with more than one the results are fp32
-// partial tiles at out + range * Mo * No (PART), else they are written as bf16 (P = 1) or fp32 (P = 3).
+// partial tiles at out + range * Mo * No (OUT_PART).
 //
 // What bounds it with many rows is the way of the operands into LDS: with 128 x 128 tiles the weight
 // gradient 2048 x 256 over 146689 rows takes 261 us for the loads alone, 100 us for the products alone
@@ -196,19 +196,22 @@ template <int TM, int TN> struct Waves {                     // wavefronts of a 
     static constexpr int NW = TM * TN >= 256 * 128 ? 8 : 4;
     static constexpr int WM = NW == 4 || TM <= TN ? 2 : 4, WN = NW / WM;
 };
-template <int P, int TM, int TN, bool PART> struct GemmLds {
+// results: fp32 partial tiles of a range of the contraction, or the product itself in bf16 or fp32
+enum : int { OUT_BF16 = KFH_BF16, OUT_F32 = KFH_F32, OUT_PART };
+template <int P, int TM, int TN, int OUT> struct GemmLds {
     static constexpr int BK = P == 3 ? 32 : 64, NT = Waves<TM, TN>::NW * 64;
-    using Out = TileStore<PART || P == 3 ? (int)KFH_F32 : (int)KFH_BF16, TM, TN / Waves<TM, TN>::WN, NT>;  // one column of wavefronts
+    using Out = TileStore<OUT == OUT_BF16 ? (int)KFH_BF16 : (int)KFH_F32, TM, TN / Waves<TM, TN>::WN, NT>;  // one column of wavefronts
     static constexpr int IN = 2 * P * (TM + TN) * (BK + 8) * 2;
     static constexpr int BYTES = IN > Out::BYTES ? IN : Out::BYTES;
 };
 
-template <int P, int AK, int BK_, bool PART, int TM, int TN>
+template <int P, int AK, int BK_, int OUT, int TM, int TN>
 __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
     const void* __restrict__ A, long long lda, long long ap, const void* __restrict__ B, long long ldb, long long bp,
     void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits) {
     using W = Waves<TM, TN>;
-    using Lds = GemmLds<P, TM, TN, PART>;
+    using Lds = GemmLds<P, TM, TN, OUT>;
+    constexpr bool PART = OUT == OUT_PART;
     constexpr int BK = Lds::BK, LDK = BK + 8, NT = Lds::NT;
     constexpr int RM = TM / W::WM, RN = TN / W::WN, NA = RM / 32, NB = RN / 32;
     // k-tiles on their way in registers: the small tiles are used where there are few workgroups and the
@@ -372,15 +375,18 @@ __global__ __launch_bounds__(64 * kSmallWaves) void ffn_small_kernel(const uint1
     if (m0 + col < M && n < N) store4<KFH_BF16>(out, (size_t)(m0 + col) * N + n, o[0][0], o[0][1], o[0][2], o[0][3]);
 }
 
-// out[i] = sum of `parts` fp32 values part[z * n + i]: 64 lanes x 4 values per workgroup, its four
-// wavefronts take every fourth part; a fixed order
-__global__ __launch_bounds__(256) void ffn_sum_parts_kernel(const float* __restrict__ part, int parts, long long n,
-                                                            void* __restrict__ out, int out_dtype) {
+// out[i] = sum of `parts` fp32 values part[z * n + i], for up to two results (blockIdx.y): 64 lanes x 4
+// values per workgroup, its four wavefronts take every fourth part; a fixed order
+struct SumArgs { const float* part[2]; int parts[2]; long long n[2]; void* out[2]; };
+template <int IO>
+__global__ __launch_bounds__(256) void ffn_sum_parts_kernel(SumArgs p) {
     __shared__ f32x4 red[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long i = ((long long)blockIdx.x * 64 + lane) * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
+    const long long i = ((long long)blockIdx.x * 64 + lane) * 4, n = p.n[t];
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (i < n) {
+        const float* const part = p.part[t];
+        const int parts = p.parts[t];
 #pragma unroll 4
         for (int z = wave; z < parts; z += 4) {
             const f32x4 w = *reinterpret_cast<const f32x4*>(part + (size_t)z * n + i);
@@ -394,8 +400,7 @@ __global__ __launch_bounds__(256) void ffn_sum_parts_kernel(const float* __restr
     float o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = (red[0][lane][e] + red[1][lane][e]) + (red[2][lane][e] + red[3][lane][e]);
-    if (out_dtype == KFH_BF16) store4<KFH_BF16>(out, (size_t)i, o[0], o[1], o[2], o[3]);
-    else store4<KFH_F32>(out, (size_t)i, o[0], o[1], o[2], o[3]);
+    store4<IO>(p.out[t], (size_t)i, o[0], o[1], o[2], o[3]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -423,15 +428,16 @@ static Wgrad wgrad_plan(long long M, long long a, long long b, int io_dtype) {
     const long long most = max(1LL, up_div(M, 256));
     w.t = pick_tile(a, b, most, io_dtype);
     const long long tiles = up_div(a, w.t.m) * up_div(b, w.t.n);
-    w.splits = (int)min(min(max(1LL, (w.t.m * w.t.n > 128 * 128 ? 256 : 512) / tiles), most), 256LL);
+    // (two at least where there are rows for two: one range means few rows, and no partial sums)
+    w.splits = (int)min(min(max(2LL, (w.t.m * w.t.n > 128 * 128 ? 256 : 512) / tiles), most), 256LL);
     if (w.splits > 8) w.splits = w.splits / 8 * 8;           // whole rounds over the XCDs
     w.per = up_div(up_div(M, w.splits), 64) * 64;
     return w;
 }
-static size_t wgrad_part_bytes(long long M, int C, int F, int io_dtype) {
-    const size_t a = (size_t)wgrad_plan(M, 2LL * F, C, io_dtype).splits * 2 * F * C * 4;
-    const size_t b = (size_t)wgrad_plan(M, C, F, io_dtype).splits * F * C * 4;
-    return a > b ? a : b;
+// (one range needs no partial sums)
+static size_t wgrad_part_bytes(long long M, long long a, long long b, int io_dtype) {
+    const int s = wgrad_plan(M, a, b, io_dtype).splits;
+    return s > 1 ? (size_t)s * a * b * 4 : 0;
 }
 
 // A product with few tiles and a long contraction is cut into ranges of it (at least 8 k-tiles each, from
@@ -459,7 +465,7 @@ static bool few_rows(long long M, int F) { return up_div(M, 64) * up_div(F, 64) 
 
 // Workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F], row-major in P planes or (streamed)
 // in blocks; packed weights of the streamed kernels; planes of x, w_in, w_out and dy (fp32); partial sums
-struct FfnWs { size_t h, d, pack, x, wi, wo, dy, part, total; };
+struct FfnWs { size_t h, d, pack, x, wi, wo, dy, part, part_wi, part_wo, total; };
 static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     const size_t e = io_dtype == KFH_F32 ? 6 : 2, split = io_dtype == KFH_F32 ? 6 : 0;
     const bool st = streamed(M, C, F, io_dtype), fused = st && C <= 128;
@@ -474,9 +480,9 @@ static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     w.wi = take((size_t)2 * F * C * split);
     w.wo = take((size_t)F * C * split);
     w.dy = take(backward ? (size_t)M * C * split : 0);
-    size_t part = fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype);
-    if (backward) part = max(part, wgrad_part_bytes(M, C, F, io_dtype));
-    w.part = take(part);
+    w.part = take(fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype));
+    w.part_wi = take(backward ? wgrad_part_bytes(M, 2LL * F, C, io_dtype) : 0);
+    w.part_wo = take(backward ? wgrad_part_bytes(M, C, F, io_dtype) : 0);
     w.total = at;
     return w;
 }
@@ -484,10 +490,21 @@ size_t gated_ffn_ws_bytes(long long M, int C, int F, int backward, int io_dtype)
     return ffn_ws(M, C, F, backward, io_dtype).total;
 }
 
-static void sum_parts(const float* part, int parts, long long n, void* out, int out_dtype, hipStream_t stream) {
-    hipLaunchKernelGGL(ffn_sum_parts_kernel, dim3((unsigned)up_div(n, 256)), dim3(256), 0, stream, part, parts, n, out,
-                       out_dtype);
-}
+// the sums of the results that have partial sums (parts > 1)
+struct Sums {
+    SumArgs a;
+    int count = 0;
+    void add(const float* part, int parts, long long n, void* out) {
+        a.part[count] = part; a.parts[count] = parts; a.n[count] = n; a.out[count] = out;
+        ++count;
+    }
+    void run(int out_dtype, hipStream_t stream) const {
+        if (count == 0) return;
+        const dim3 grid((unsigned)up_div(count > 1 ? max(a.n[0], a.n[1]) : a.n[0], 256), (unsigned)count);
+        if (out_dtype == KFH_BF16) hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_BF16>, grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_F32>, grid, dim3(256), 0, stream, a);
+    }
+};
 
 template <int P, bool BWD>
 static void hidden(const void* x, const void* dy, const void* w_in, const void* w_out, void* h, void* d, long long M, int C,
@@ -508,12 +525,12 @@ static void hidden(const void* x, const void* dy, const void* w_in, const void* 
 // an operand: its first part, elements per row, bytes between parts
 struct Operand { const void* p; long long ld, plane; };
 
-template <int P, int AK, int BK_, bool PART, int TM, int TN>
+template <int P, int AK, int BK_, int OUT, int TM, int TN>
 static void gemm(Operand a, Operand b, void* out, long long Mo, int No, long long K, long long kper, int splits,
                  hipStream_t stream) {
     const long long mt = up_div(Mo, TM), nt = up_div(No, TN);
-    hipLaunchKernelGGL((ffn_gemm_kernel<P, AK, BK_, PART, TM, TN>),
-                       dim3(PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(Waves<TM, TN>::NW * 64), 0,
+    hipLaunchKernelGGL((ffn_gemm_kernel<P, AK, BK_, OUT, TM, TN>),
+                       dim3(OUT == OUT_PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(Waves<TM, TN>::NW * 64), 0,
                        stream, a.p, a.ld, a.plane, b.p, b.ld, b.plane, out, Mo, No, K, kper, splits);
 }
 
@@ -523,31 +540,40 @@ static void product(Operand a, Operand b, void* out, float* part, long long Mo, 
     constexpr int IO = P == 3 ? KFH_F32 : KFH_BF16;
     const Tile t = pick_tile(Mo, No, 1, IO);
     if constexpr (AK == K_BLOCK) {                          // streamed calls: 16384 rows of 256 channels at least
-        if (t.m == 256) gemm<P, AK, BK_, false, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
-        else gemm<P, AK, BK_, false, 128, 128>(a, b, out, Mo, No, K, K, 1, stream);
+        if (t.m == 256) gemm<P, AK, BK_, IO, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
+        else gemm<P, AK, BK_, IO, 128, 128>(a, b, out, Mo, No, K, K, 1, stream);
     } else {
         const int splits = product_splits(Mo, No, K, IO);
         if (splits > 1) {
             const long long BK = P == 3 ? 32 : 64, per = up_div(up_div(K, BK), splits) * BK;
-            gemm<P, AK, BK_, true, 64, 64>(a, b, part, Mo, No, K, per, splits, stream);
-            return sum_parts(part, splits, Mo * No, out, IO, stream);
+            gemm<P, AK, BK_, OUT_PART, 64, 64>(a, b, part, Mo, No, K, per, splits, stream);
+            Sums s;
+            s.add(part, splits, Mo * No, out);
+            return s.run(IO, stream);
         }
         if constexpr (P == 1) {
-            if (t.n == 256) return gemm<P, AK, BK_, false, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
-            if (t.m == 256) return gemm<P, AK, BK_, false, 256, 128>(a, b, out, Mo, No, K, K, 1, stream);
-            if (t.m == 128) return gemm<P, AK, BK_, false, 128, 128>(a, b, out, Mo, No, K, K, 1, stream);
+            if (t.n == 256) return gemm<P, AK, BK_, IO, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
+            if (t.m == 256) return gemm<P, AK, BK_, IO, 256, 128>(a, b, out, Mo, No, K, K, 1, stream);
+            if (t.m == 128) return gemm<P, AK, BK_, IO, 128, 128>(a, b, out, Mo, No, K, K, 1, stream);
         }
-        gemm<P, AK, BK_, false, 64, 64>(a, b, out, Mo, No, K, K, 1, stream);
+        gemm<P, AK, BK_, IO, 64, 64>(a, b, out, Mo, No, K, K, 1, stream);
     }
 }
 
-// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]; AK, BK_: R_MAJOR or R_BLOCK
+// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]; AK, BK_: R_MAJOR or R_BLOCK.  Partial sums are left to `sums`.
 template <int P, int AK, int BK_>
-static void wgrad(Operand a, int Ma, Operand b, int Nb, float* part, void* out, int out_dtype, long long M,
+static void wgrad(Operand a, int Ma, Operand b, int Nb, float* part, void* out, int out_dtype, long long M, Sums& sums,
                   hipStream_t stream) {
     const Wgrad w = wgrad_plan(M, Ma, Nb, P == 3 ? KFH_F32 : KFH_BF16);
+    if constexpr (AK == R_MAJOR && BK_ == R_MAJOR) {        // (streamed calls have rows for more than one range)
+        if (w.splits == 1) {
+            if (out_dtype == KFH_BF16) gemm<P, AK, BK_, OUT_BF16, 64, 64>(a, b, out, Ma, Nb, M, w.per, 1, stream);
+            else gemm<P, AK, BK_, OUT_F32, 64, 64>(a, b, out, Ma, Nb, M, w.per, 1, stream);
+            return;
+        }
+    }
     auto run = [&](auto tm, auto tn) {
-        gemm<P, AK, BK_, true, decltype(tm)::v, decltype(tn)::v>(a, b, part, Ma, Nb, M, w.per, w.splits, stream);
+        gemm<P, AK, BK_, OUT_PART, decltype(tm)::v, decltype(tn)::v>(a, b, part, Ma, Nb, M, w.per, w.splits, stream);
     };
     bool done = false;
     if constexpr (P == 1) {
@@ -559,7 +585,7 @@ static void wgrad(Operand a, int Ma, Operand b, int Nb, float* part, void* out, 
         else done = false;
     }
     if (!done) run(Int<64>{}, Int<64>{});
-    sum_parts(part, w.splits, (long long)Ma * Nb, out, out_dtype, stream);
+    sums.add(part, w.splits, (long long)Ma * Nb, out);
 }
 
 // the three planes of the fp32 operands
@@ -616,6 +642,9 @@ static void backward_t(const void* dy, const void* x, const void* w_in, const vo
     char* const h = ws + w.h;
     char* const d = ws + w.d;
     float* const part = reinterpret_cast<float*>(ws + w.part);
+    float* const part_wi = reinterpret_cast<float*>(ws + w.part_wi);
+    float* const part_wo = reinterpret_cast<float*>(ws + w.part_wo);
+    Sums sums;
     if constexpr (P == 3) {
         split_operands(x, w_in, w_out, dy, ws, w, M, C, F, stream);
         x = ws + w.x;
@@ -624,15 +653,17 @@ static void backward_t(const void* dy, const void* x, const void* w_in, const vo
         dy = ws + w.dy;
     } else if (streamed(M, C, F, KFH_BF16)) {
         launch_ffn_stream(x, dy, w_in, w_out, ws + w.pack, h, d, dx, M, C, F, stream);
-        if (dw_out) wgrad<1, R_MAJOR, R_BLOCK>({dy, C, 0}, C, {h, F, 0}, F, part, dw_out, dw_dtype, M, stream);
-        if (dw_in) wgrad<1, R_BLOCK, R_MAJOR>({d, 2LL * F, 0}, 2 * F, {x, C, 0}, C, part, dw_in, dw_dtype, M, stream);
+        if (dw_out) wgrad<1, R_MAJOR, R_BLOCK>({dy, C, 0}, C, {h, F, 0}, F, part_wo, dw_out, dw_dtype, M, sums, stream);
+        if (dw_in) wgrad<1, R_BLOCK, R_MAJOR>({d, 2LL * F, 0}, 2 * F, {x, C, 0}, C, part_wi, dw_in, dw_dtype, M, sums, stream);
+        sums.run(dw_dtype, stream);
         if (dx && C > 128) product<1, K_BLOCK, R_MAJOR>({d, 2LL * F, 0}, {w_in, C, 0}, dx, part, M, C, 2LL * F, stream);
         return;
     }
     hidden<P, true>(x, dy, w_in, w_out, h, d, M, C, F, stream);
     const Operand X = {x, C, M * C * 2}, DY = {dy, C, M * C * 2}, H = {h, F, M * F * 2}, D = {d, 2LL * F, M * 2 * F * 2};
-    if (dw_out) wgrad<P, R_MAJOR, R_MAJOR>(DY, C, H, F, part, dw_out, dw_dtype, M, stream);
-    if (dw_in) wgrad<P, R_MAJOR, R_MAJOR>(D, 2 * F, X, C, part, dw_in, dw_dtype, M, stream);
+    if (dw_out) wgrad<P, R_MAJOR, R_MAJOR>(DY, C, H, F, part_wo, dw_out, dw_dtype, M, sums, stream);
+    if (dw_in) wgrad<P, R_MAJOR, R_MAJOR>(D, 2 * F, X, C, part_wi, dw_in, dw_dtype, M, sums, stream);
+    sums.run(dw_dtype, stream);
     if (dx) product<P, K_MAJOR, R_MAJOR>(D, {w_in, C, 4LL * F * C}, dx, part, M, C, 2LL * F, stream);
 }
 
