@@ -70,22 +70,27 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
                                                                   uint16_t* __restrict__ d, uint16_t* __restrict__ out, long long M,
                                                                   int F) {
     constexpr int C = 16 * KS, NF = stream_frags<KS, BWD, FUSE>(), NT = NW * 64, NB = FUSE ? KS / 2 : 1;
-    constexpr int SLOTS = NF * 64, NPRE = (SLOTS + NT - 1) / NT;
+    // backward: the weights of the next step come in two halves, one during the first products and one during
+    // the activation and the second products, with half the registers on the way (147456 x 128 x 256: 179 ->
+    // 162 us); forward: during the activation and the second products
+    constexpr int SLOTS = NF * 64, NPRE = (SLOTS + NT - 1) / NT, H0 = BWD ? (NPRE + 1) / 2 : NPRE;
     __shared__ __attribute__((aligned(16))) u32x4 smem[2 * SLOTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
     const long long p0 = (long long)blockIdx.x * (32 * NW) + wave * 32;
     const int steps = F / 32;
-    u32x4 pre[NPRE];
-    auto fetch = [&](int s) {
+    u32x4 pre[H0];
+    auto fetch = [&](int s, auto part) {
+        constexpr int I0 = decltype(part)::v ? H0 : 0, I1 = decltype(part)::v ? NPRE : H0;
 #pragma unroll
-        for (int i = 0; i < NPRE; ++i) pre[i] = wp[(size_t)s * SLOTS + min(i * NT + tid, SLOTS - 1)];
+        for (int i = I0; i < I1; ++i) pre[i - I0] = wp[(size_t)s * SLOTS + (SLOTS % NT ? min(i * NT + tid, SLOTS - 1) : i * NT + tid)];
     };
-    auto commit = [&](int b) {
+    auto commit = [&](int b, auto part) {
+        constexpr int I0 = decltype(part)::v ? H0 : 0, I1 = decltype(part)::v ? NPRE : H0;
 #pragma unroll
-        for (int i = 0; i < NPRE; ++i)
-            if (SLOTS % NT == 0 || i * NT + tid < SLOTS) smem[b * SLOTS + i * NT + tid] = pre[i];
+        for (int i = I0; i < I1; ++i)
+            if (SLOTS % NT == 0 || i * NT + tid < SLOTS) smem[b * SLOTS + i * NT + tid] = pre[i - I0];
     };
-    fetch(0);
+    fetch(0, Int<0>{});
     const long long p = p0 + col;
     const bool live = p < M;
     const size_t row = (size_t)min(p, M - 1) * C + 8 * half;
@@ -96,7 +101,9 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) yf[ks] = *reinterpret_cast<const bf16x8*>(dy + row + 16 * ks);
     }
-    commit(0);
+    commit(0, Int<0>{});
+    fetch(0, Int<1>{});
+    commit(0, Int<1>{});
     __syncthreads();
     f32x16 oacc[NB];
     if constexpr (FUSE) {
@@ -161,11 +168,21 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
         }
     };
     for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) fetch(s + 1);
+        if (BWD && s + 1 < steps) fetch(s + 1, Int<0>{});
         const bf16x8* w = reinterpret_cast<const bf16x8*>(smem + (s & 1) * SLOTS) + lane;
+        __builtin_amdgcn_s_setprio(1);        // before the wavefronts that are in their activations: 1-3 %
         products(w);
+        __builtin_amdgcn_s_setprio(0);
+        if (s + 1 < steps) {
+            if constexpr (BWD) {
+                commit((s + 1) & 1, Int<0>{});
+                fetch(s + 1, Int<1>{});
+            } else {
+                fetch(s + 1, Int<0>{});
+            }
+        }
         finish(s, w);
-        if (s + 1 < steps) commit((s + 1) & 1);
+        if (s + 1 < steps) commit((s + 1) & 1, Int<(BWD ? 1 : 0)>{});
         __syncthreads();
     }
     if constexpr (FUSE) {

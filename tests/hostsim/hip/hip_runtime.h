@@ -200,6 +200,7 @@ inline size_t max(size_t a, size_t b) { return a > b ? a : b; }
 #define __builtin_amdgcn_wave_barrier() ::hostsim::wave_barrier()
 #define __builtin_amdgcn_s_waitcnt(x) ((void)0)
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
+#define __builtin_amdgcn_s_setprio(x) ((void)0)
 #define __builtin_amdgcn_sched_group_barrier(a, b, c) ((void)0)
 #define __builtin_amdgcn_rsqf(x) (1.0f / sqrtf((x)))
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
