@@ -540,7 +540,9 @@ static void product(Operand a, Operand b, void* out, float* part, long long Mo, 
     constexpr int IO = P == 3 ? KFH_F32 : KFH_BF16;
     const Tile t = pick_tile(Mo, No, 1, IO);
     if constexpr (AK == K_BLOCK) {                          // streamed calls: 16384 rows of 256 channels at least
-        if (t.m == 256) gemm<P, AK, BK_, IO, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
+        // (y: 128 rows a tile, 256 leave the compiler three registers short)
+        constexpr int TM = BK_ == K_MAJOR ? 128 : 256;
+        if (t.m == 256) gemm<P, AK, BK_, IO, TM, 256>(a, b, out, Mo, No, K, K, 1, stream);
         else gemm<P, AK, BK_, IO, 128, 128>(a, b, out, Mo, No, K, K, 1, stream);
     } else {
         const int splits = product_splits(Mo, No, K, IO);
