@@ -20,6 +20,15 @@ DEV = "cuda:0"
 VECTORS = Path(__file__).resolve().parent / "golden" / "host_model_vectors.pt"
 MIN_IDENTICAL = 0.9          # expected: > 0.999 (see the module docstring)
 
+# Largest difference of a bf16 output, in units of compare().  An output y_i = sum_j W_ij o_j of the token
+# attention (768 terms) is made of values o_j that both sides round to bf16; where the fp32 value lies
+# next to a rounding border the two take neighbours, at most 2^-7 |o_j| apart.  With a share f of such o_j,
+# of either sign, the variance of y_i's difference is at most f 2^-14 sum_j W_ij^2 o_j^2 = f 2^-14 RMS(y)^2;
+# for f = 1 - MIN_IDENTICAL = 0.1 the standard deviation is 2.5e-3 RMS(y).  Five of them (the largest of the
+# 61440 values of the case lies at 4.3) are 1.24e-2 RMS(y).  A unit is at least the bf16 spacing at RMS(y) / 16,
+# which is no less than 2^-8 / 16 RMS(y) = 2.44e-4 RMS(y): 1.24e-2 / 2.44e-4 = 51 units.
+MAX_UNITS = 51
+
 
 def compare(dev) -> dict:
     """{case: (fraction of bit-identical values, largest difference in units of the value's bf16
@@ -55,4 +64,4 @@ def test_gpu_results_against_the_host_builds():
             assert worst <= 200, (name, frac, worst)          # 2e-4 of the value: fp32 arithmetic on both sides
         else:
             assert frac >= MIN_IDENTICAL, (name, frac, worst)
-            assert worst <= 16, (name, frac, worst)           # a few bf16 steps at most
+            assert worst <= MAX_UNITS, (name, frac, worst)
