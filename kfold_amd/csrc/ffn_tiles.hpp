@@ -208,8 +208,7 @@ __device__ __forceinline__ void store4(void* base, size_t e, float a, float b, f
 }
 
 // Workgroups are dealt to the 8 XCDs in turn, each with an L2 of its own: the `nt` tiles that share a
-// row tile follow each other on one XCD, so its rows are read from memory once (without it the weight
-// gradient 2048 x 256 over 146689 rows took 287 us instead of 198).  With few row tiles, unless they
+// row tile follow each other on one XCD, so its rows are read from memory once.  With few row tiles, unless they
 // divide evenly, that would leave XCDs idle, and the tiles are simply counted through.
 __host__ __device__ constexpr bool xcd_dealt(long long mtiles) { return mtiles >= 64 || mtiles % 8 == 0; }
 __device__ __forceinline__ bool xcd_tile(long long id, long long mtiles, int nt, long long& mt, int& n) {

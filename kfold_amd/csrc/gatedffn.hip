@@ -185,8 +185,9 @@ __global__ __launch_bounds__(256) void ffn_hidden_kernel(const uint16_t* __restr
 // ---------------------------------------------------------------------------------------------
 // out[m][n] = sum_k A(m, k) B(n, k), operands in P parts (planes `ap`, `bp` bytes apart); AK / BK_ as
 // TileLoad's KIND; a workgroup of NW wavefronts owns TM x TN results, wavefront (wm, wn) TM / WM x TN / WN
-// of them.  The contraction is cut into `splits` ranges of kper; with more than one the results are fp32
-// partial tiles at out + range * Mo * No (OUT_PART).
+// of them.  The contraction is cut into `splits` ranges of kper; with OUT_PART the results are fp32 partial
+// tiles at out + range * (Mo + Mo2) * No, and Mo2 more rows may come from a second pair of operands of the same
+// kinds (both weight gradients in one launch).
 //
 // What bounds it with many rows is the way of the operands into LDS: with 128 x 128 tiles the weight
 // gradient 2048 x 256 over 146689 rows takes 261 us for the loads alone, 100 us for the products alone
@@ -208,7 +209,8 @@ template <int P, int TM, int TN, int OUT> struct GemmLds {
 template <int P, int AK, int BK_, int OUT, int TM, int TN>
 __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
     const void* __restrict__ A, long long lda, long long ap, const void* __restrict__ B, long long ldb, long long bp,
-    void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits) {
+    void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits, const void* __restrict__ A2,
+    long long lda2, long long ap2, const void* __restrict__ B2, int Mo2) {
     using W = Waves<TM, TN>;
     using Lds = GemmLds<P, TM, TN, OUT>;
     constexpr bool PART = OUT == OUT_PART;
@@ -222,7 +224,7 @@ __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
     uint16_t* const buf = reinterpret_cast<uint16_t*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave % W::WM, wn = wave / W::WM;
-    const long long mtiles = (Mo + TM - 1) / TM;
+    const long long mtiles1 = (Mo + TM - 1) / TM, mtiles = mtiles1 + (PART ? (Mo2 + TM - 1) / TM : 0);
     const int ntiles = (No + TN - 1) / TN;
     // tiles that share operand rows follow each other on one XCD: those of a row tile, or (PART) all
     // tiles of one range of the contraction
@@ -235,6 +237,12 @@ __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
         nt = t % ntiles;
     } else {
         if (!xcd_tile(blockIdx.x, mtiles, ntiles, mt, nt)) return;
+    }
+    char* base = static_cast<char*>(out) + (PART ? (size_t)z * (Mo + Mo2) * No * 4 : 0);
+    if (PART && mt >= mtiles1) {
+        mt -= mtiles1;
+        base += (size_t)Mo * No * 4;
+        A = A2; lda = lda2; ap = ap2; B = B2; Mo = Mo2;
     }
     const long long m0 = mt * TM;
     const int n0 = nt * TN;
@@ -289,7 +297,6 @@ __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
     }
     // through LDS, one column of wavefronts at a time
     using Out = typename Lds::Out;
-    char* const base = static_cast<char*>(out) + (PART ? (size_t)z * Mo * No * 4 : 0);
 #pragma unroll 1
     for (int c = 0; c < W::WN; ++c) {
         if (c) __syncthreads();
@@ -375,32 +382,44 @@ __global__ __launch_bounds__(64 * kSmallWaves) void ffn_small_kernel(const uint1
     if (m0 + col < M && n < N) store4<KFH_BF16>(out, (size_t)(m0 + col) * N + n, o[0][0], o[0][1], o[0][2], o[0][3]);
 }
 
-// out[i] = sum of `parts` fp32 values part[z * n + i], for up to two results (blockIdx.y): 64 lanes x 4
-// values per workgroup, its four wavefronts take every fourth part; a fixed order
-struct SumArgs { const float* part[2]; int parts[2]; long long n[2]; void* out[2]; };
+// Sums of `parts` partial matrices [R1 + R2, C]: the first R1 rows go to out1 as they are, the other R2 rows
+// transposed to out2 [C, R2]; either may be null.  32 x 32 values per workgroup, its four groups of 256 threads take
+// every fourth part; a fixed order.
+struct SumArgs { const float* part; int parts; long long R1; int R2, C; void* out1; void* out2; };
 template <int IO>
-__global__ __launch_bounds__(256) void ffn_sum_parts_kernel(SumArgs p) {
-    __shared__ f32x4 red[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
-    const long long i = ((long long)blockIdx.x * 64 + lane) * 4, n = p.n[t];
+__global__ __launch_bounds__(1024) void ffn_sum_parts_kernel(SumArgs p) {
+    __shared__ float red[4][32][36];
+    const int t = threadIdx.x & 255, grp = threadIdx.x >> 8;
+    const long long tiles1 = (p.R1 + 31) / 32;
+    const bool second = blockIdx.y >= tiles1;
+    const long long r0 = (second ? blockIdx.y - tiles1 : (long long)blockIdx.y) * 32, rows = second ? p.R2 : p.R1;
+    const int c0 = blockIdx.x * 32, rr = t >> 3, cc = (t & 7) * 4;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (i < n) {
-        const float* const part = p.part[t];
-        const int parts = p.parts[t];
+    if (r0 + rr < rows && c0 + cc < p.C) {
+        const size_t n = (size_t)(p.R1 + p.R2) * p.C, at = (size_t)((second ? p.R1 : 0) + r0 + rr) * p.C + c0 + cc;
 #pragma unroll 4
-        for (int z = wave; z < parts; z += 4) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(part + (size_t)z * n + i);
+        for (int z = grp; z < p.parts; z += 4) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(p.part + z * n + at);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[e] += w[e];
         }
     }
-    red[wave][lane] = s;
+    *reinterpret_cast<f32x4*>(&red[grp][rr][cc]) = s;
     __syncthreads();
-    if (wave != 0 || i >= n) return;
+    if (grp != 0) return;
     float o[4];
+    if (!second) {
+        if (!p.out1 || r0 + rr >= rows || c0 + cc >= p.C) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = (red[0][lane][e] + red[1][lane][e]) + (red[2][lane][e] + red[3][lane][e]);
-    store4<IO>(p.out[t], (size_t)i, o[0], o[1], o[2], o[3]);
+        for (int e = 0; e < 4; ++e) o[e] = (red[0][rr][cc + e] + red[1][rr][cc + e]) + (red[2][rr][cc + e] + red[3][rr][cc + e]);
+        store4<IO>(p.out1, (size_t)(r0 + rr) * p.C + c0 + cc, o[0], o[1], o[2], o[3]);
+    } else {
+        // column rr of the tile, its rows cc .. cc + 3
+        if (!p.out2 || r0 + cc >= rows || c0 + rr >= p.C) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (red[0][cc + e][rr] + red[1][cc + e][rr]) + (red[2][cc + e][rr] + red[3][cc + e][rr]);
+        store4<IO>(p.out2, (size_t)(c0 + rr) * p.R2 + r0 + cc, o[0], o[1], o[2], o[3]);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -420,24 +439,24 @@ static Tile pick_tile(long long a, long long b, long long more, int io_dtype) {
     return {64, 64};
 }
 
-// Ranges of rows the weight gradients are summed over in parallel: one workgroup per CU with large tiles (as
-// many as fit; more would only add partial sums), two with the others, at least 256 rows each.
+// Both weight gradients are one product [2F + F, C] over the rows: (du, dv)^T x and h^T dy.  Ranges of rows that are
+// summed in parallel: one workgroup per CU with large tiles (as many as fit; more would only add partial sums),
+// two with the others, at least 256 rows each.
 struct Wgrad { Tile t; int splits; long long per; };
-static Wgrad wgrad_plan(long long M, long long a, long long b, int io_dtype) {
+static Wgrad wgrad_plan(long long M, long long a1, long long a2, long long b, int io_dtype) {
     Wgrad w;
     const long long most = max(1LL, up_div(M, 256));
-    w.t = pick_tile(a, b, most, io_dtype);
-    const long long tiles = up_div(a, w.t.m) * up_div(b, w.t.n);
-    // (two at least where there are rows for two: one range means few rows, and no partial sums)
-    w.splits = (int)min(min(max(2LL, (w.t.m * w.t.n > 128 * 128 ? 256 : 512) / tiles), most), 256LL);
-    if (w.splits > 8) w.splits = w.splits / 8 * 8;           // whole rounds over the XCDs
+    w.t = pick_tile(a1 + a2, b, most, io_dtype);
+    const long long tiles = (up_div(a1, w.t.m) + up_div(a2, w.t.m)) * up_div(b, w.t.n);
+    w.splits = (int)min(min(max(1LL, (w.t.m * w.t.n > 128 * 128 ? 256 : 512) / tiles), most), 256LL);
+    // whole rounds over the XCDs, unless more than a tenth of the workgroups went (2048 + 1024 channels of d and h
+    // by 256, 21 ranges: 313 us counted through, 362 with 16 ranges dealt to the XCDs; 146689 rows)
+    if (const int r = w.splits / 8 * 8; r * 10 >= w.splits * 9) w.splits = r;
     w.per = up_div(up_div(M, w.splits), 64) * 64;
     return w;
 }
-// (one range needs no partial sums)
-static size_t wgrad_part_bytes(long long M, long long a, long long b, int io_dtype) {
-    const int s = wgrad_plan(M, a, b, io_dtype).splits;
-    return s > 1 ? (size_t)s * a * b * 4 : 0;
+static size_t wgrad_part_bytes(long long M, int C, int F, int io_dtype) {
+    return (size_t)wgrad_plan(M, 2LL * F, F, C, io_dtype).splits * 3 * F * C * 4;
 }
 
 // A product with few tiles and a long contraction is cut into ranges of it (at least 8 k-tiles each, from
@@ -465,7 +484,7 @@ static bool few_rows(long long M, int F) { return up_div(M, 64) * up_div(F, 64) 
 
 // Workspace: h [M, F] (not in a fused forward call), backward: d [M, 2F], row-major in P planes or (streamed)
 // in blocks; packed weights of the streamed kernels; planes of x, w_in, w_out and dy (fp32); partial sums
-struct FfnWs { size_t h, d, pack, x, wi, wo, dy, part, part_wi, part_wo, total; };
+struct FfnWs { size_t h, d, pack, x, wi, wo, dy, part, total; };
 static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     const size_t e = io_dtype == KFH_F32 ? 6 : 2, split = io_dtype == KFH_F32 ? 6 : 0;
     const bool st = streamed(M, C, F, io_dtype), fused = st && C <= 128;
@@ -480,9 +499,10 @@ static FfnWs ffn_ws(long long M, int C, int F, int backward, int io_dtype) {
     w.wi = take((size_t)2 * F * C * split);
     w.wo = take((size_t)F * C * split);
     w.dy = take(backward ? (size_t)M * C * split : 0);
-    w.part = take(fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype));
-    w.part_wi = take(backward ? wgrad_part_bytes(M, 2LL * F, C, io_dtype) : 0);
-    w.part_wo = take(backward ? wgrad_part_bytes(M, C, F, io_dtype) : 0);
+    // (the weight gradients' and the product's one after the other)
+    size_t part = fused ? 0 : product_part_bytes(M, C, backward ? 2LL * F : F, io_dtype);
+    if (backward) part = max(part, wgrad_part_bytes(M, C, F, io_dtype));
+    w.part = take(part);
     w.total = at;
     return w;
 }
@@ -490,21 +510,11 @@ size_t gated_ffn_ws_bytes(long long M, int C, int F, int backward, int io_dtype)
     return ffn_ws(M, C, F, backward, io_dtype).total;
 }
 
-// the sums of the results that have partial sums (parts > 1)
-struct Sums {
-    SumArgs a;
-    int count = 0;
-    void add(const float* part, int parts, long long n, void* out) {
-        a.part[count] = part; a.parts[count] = parts; a.n[count] = n; a.out[count] = out;
-        ++count;
-    }
-    void run(int out_dtype, hipStream_t stream) const {
-        if (count == 0) return;
-        const dim3 grid((unsigned)up_div(count > 1 ? max(a.n[0], a.n[1]) : a.n[0], 256), (unsigned)count);
-        if (out_dtype == KFH_BF16) hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_BF16>, grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_F32>, grid, dim3(256), 0, stream, a);
-    }
-};
+static void sum_parts(const SumArgs& a, int out_dtype, hipStream_t stream) {
+    const dim3 grid((unsigned)up_div(a.C, 32), (unsigned)(up_div(a.R1, 32) + up_div(a.R2, 32)));
+    if (out_dtype == KFH_BF16) hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_BF16>, grid, dim3(1024), 0, stream, a);
+    else hipLaunchKernelGGL(ffn_sum_parts_kernel<KFH_F32>, grid, dim3(1024), 0, stream, a);
+}
 
 template <int P, bool BWD>
 static void hidden(const void* x, const void* dy, const void* w_in, const void* w_out, void* h, void* d, long long M, int C,
@@ -527,11 +537,11 @@ struct Operand { const void* p; long long ld, plane; };
 
 template <int P, int AK, int BK_, int OUT, int TM, int TN>
 static void gemm(Operand a, Operand b, void* out, long long Mo, int No, long long K, long long kper, int splits,
-                 hipStream_t stream) {
-    const long long mt = up_div(Mo, TM), nt = up_div(No, TN);
+                 hipStream_t stream, Operand a2 = {}, Operand b2 = {}, int Mo2 = 0) {
+    const long long mt = up_div(Mo, TM) + up_div(Mo2, TM), nt = up_div(No, TN);
     hipLaunchKernelGGL((ffn_gemm_kernel<P, AK, BK_, OUT, TM, TN>),
                        dim3(OUT == OUT_PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(Waves<TM, TN>::NW * 64), 0,
-                       stream, a.p, a.ld, a.plane, b.p, b.ld, b.plane, out, Mo, No, K, kper, splits);
+                       stream, a.p, a.ld, a.plane, b.p, b.ld, b.plane, out, Mo, No, K, kper, splits, a2.p, a2.ld, a2.plane, b2.p, Mo2);
 }
 
 // out [Mo, No] = A [Mo, K] (AK) times B, [No, K] (K_MAJOR) or [K, No] (R_MAJOR); part: product_part_bytes
@@ -549,9 +559,7 @@ static void product(Operand a, Operand b, void* out, float* part, long long Mo, 
         if (splits > 1) {
             const long long BK = P == 3 ? 32 : 64, per = up_div(up_div(K, BK), splits) * BK;
             gemm<P, AK, BK_, OUT_PART, 64, 64>(a, b, part, Mo, No, K, per, splits, stream);
-            Sums s;
-            s.add(part, splits, Mo * No, out);
-            return s.run(IO, stream);
+            return sum_parts({part, splits, Mo, 0, No, out, nullptr}, IO, stream);
         }
         if constexpr (P == 1) {
             if (t.n == 256) return gemm<P, AK, BK_, IO, 256, 256>(a, b, out, Mo, No, K, K, 1, stream);
@@ -562,20 +570,17 @@ static void product(Operand a, Operand b, void* out, float* part, long long Mo, 
     }
 }
 
-// out [Ma, Nb] = A [M, Ma]^T B [M, Nb]; AK, BK_: R_MAJOR or R_BLOCK.  Partial sums are left to `sums`.
-template <int P, int AK, int BK_>
-static void wgrad(Operand a, int Ma, Operand b, int Nb, float* part, void* out, int out_dtype, long long M, Sums& sums,
-                  hipStream_t stream) {
-    const Wgrad w = wgrad_plan(M, Ma, Nb, P == 3 ? KFH_F32 : KFH_BF16);
-    if constexpr (AK == R_MAJOR && BK_ == R_MAJOR) {        // (streamed calls have rows for more than one range)
-        if (w.splits == 1) {
-            if (out_dtype == KFH_BF16) gemm<P, AK, BK_, OUT_BF16, 64, 64>(a, b, out, Ma, Nb, M, w.per, 1, stream);
-            else gemm<P, AK, BK_, OUT_F32, 64, 64>(a, b, out, Ma, Nb, M, w.per, 1, stream);
-            return;
-        }
-    }
+// dw_in [2F, C] = d^T x and dw_out [C, F] = (h^T dy)^T; d and h of kind AK (R_MAJOR or R_BLOCK); either result may
+// be null, its rows are then left out
+template <int P, int AK>
+static void wgrad(Operand d, Operand x, Operand h, Operand dy, float* part, void* dw_in, void* dw_out, int out_dtype, long long M,
+                  int C, int F, hipStream_t stream) {
+    if (!dw_in && !dw_out) return;
+    const int Ma = dw_in ? 2 * F : F, Mb = dw_in && dw_out ? F : 0;
+    const Wgrad w = wgrad_plan(M, 2LL * F, F, C, P == 3 ? KFH_F32 : KFH_BF16);
     auto run = [&](auto tm, auto tn) {
-        gemm<P, AK, BK_, OUT_PART, decltype(tm)::v, decltype(tn)::v>(a, b, part, Ma, Nb, M, w.per, w.splits, stream);
+        gemm<P, AK, R_MAJOR, OUT_PART, decltype(tm)::v, decltype(tn)::v>(dw_in ? d : h, dw_in ? x : dy, part, Ma, C, M, w.per, w.splits,
+                                                                        stream, h, dy, Mb);
     };
     bool done = false;
     if constexpr (P == 1) {
@@ -587,7 +592,8 @@ static void wgrad(Operand a, int Ma, Operand b, int Nb, float* part, void* out, 
         else done = false;
     }
     if (!done) run(Int<64>{}, Int<64>{});
-    sums.add(part, w.splits, (long long)Ma * Nb, out);
+    // (dw_out alone: no direct rows)
+    sum_parts({part, w.splits, dw_in ? 2LL * F : 0, dw_out ? F : 0, C, dw_in, dw_out}, out_dtype, stream);
 }
 
 // the three planes of the fp32 operands
@@ -644,9 +650,6 @@ static void backward_t(const void* dy, const void* x, const void* w_in, const vo
     char* const h = ws + w.h;
     char* const d = ws + w.d;
     float* const part = reinterpret_cast<float*>(ws + w.part);
-    float* const part_wi = reinterpret_cast<float*>(ws + w.part_wi);
-    float* const part_wo = reinterpret_cast<float*>(ws + w.part_wo);
-    Sums sums;
     if constexpr (P == 3) {
         split_operands(x, w_in, w_out, dy, ws, w, M, C, F, stream);
         x = ws + w.x;
@@ -655,17 +658,13 @@ static void backward_t(const void* dy, const void* x, const void* w_in, const vo
         dy = ws + w.dy;
     } else if (streamed(M, C, F, KFH_BF16)) {
         launch_ffn_stream(x, dy, w_in, w_out, ws + w.pack, h, d, dx, M, C, F, stream);
-        if (dw_out) wgrad<1, R_MAJOR, R_BLOCK>({dy, C, 0}, C, {h, F, 0}, F, part_wo, dw_out, dw_dtype, M, sums, stream);
-        if (dw_in) wgrad<1, R_BLOCK, R_MAJOR>({d, 2LL * F, 0}, 2 * F, {x, C, 0}, C, part_wi, dw_in, dw_dtype, M, sums, stream);
-        sums.run(dw_dtype, stream);
+        wgrad<1, R_BLOCK>({d, 2LL * F, 0}, {x, C, 0}, {h, F, 0}, {dy, C, 0}, part, dw_in, dw_out, dw_dtype, M, C, F, stream);
         if (dx && C > 128) product<1, K_BLOCK, R_MAJOR>({d, 2LL * F, 0}, {w_in, C, 0}, dx, part, M, C, 2LL * F, stream);
         return;
     }
     hidden<P, true>(x, dy, w_in, w_out, h, d, M, C, F, stream);
     const Operand X = {x, C, M * C * 2}, DY = {dy, C, M * C * 2}, H = {h, F, M * F * 2}, D = {d, 2LL * F, M * 2 * F * 2};
-    if (dw_out) wgrad<P, R_MAJOR, R_MAJOR>(DY, C, H, F, part_wo, dw_out, dw_dtype, M, sums, stream);
-    if (dw_in) wgrad<P, R_MAJOR, R_MAJOR>(D, 2 * F, X, C, part_wi, dw_in, dw_dtype, M, sums, stream);
-    sums.run(dw_dtype, stream);
+    wgrad<P, R_MAJOR>(D, X, H, DY, part, dw_in, dw_out, dw_dtype, M, C, F, stream);
     if (dx) product<P, K_MAJOR, R_MAJOR>(D, {w_in, C, 4LL * F * C}, dx, part, M, C, 2LL * F, stream);
 }
 
