@@ -222,7 +222,6 @@ __global__ __launch_bounds__(256) void ln_bwd_reg_kernel(const void* dy, const v
 #pragma unroll
             for (int i = 0; i < N; ++i) v[k][i] = (v[k][i] - mean[k]) * rstd[k];
             Row::trim(C, l, v[k]);
-            Row::trim(C, l, a[k]);
             if (SUMS && r0 + k * RPB < M) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -232,7 +231,9 @@ __global__ __launch_bounds__(256) void ln_bwd_reg_kernel(const void* dy, const v
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                a[k][i] *= gam[i];
+#pragma unroll
+            for (int i = 0; i < N; ++i) a[k][i] *= gam[i];
+            Row::trim(C, l, a[k]);           // (the product: 0 times an infinite weight would be NaN)
                 s1[k] += a[k][i];
                 s2[k] += a[k][i] * v[k][i];
             }

@@ -285,6 +285,26 @@ def test_gated_ffn_big_tiles(M, C, F):
         within(got, r[name], e[name], name)
 
 
+@pytest.mark.parametrize("C", [5, 40, 72, 264, 765, 768, 1544])
+def test_layer_norm_infinite_weight(C):
+    """An infinite weight of the last channel: dx is infinite and NaN exactly where the formula is (a lane
+    without channels of its own adds nothing)."""
+    print(f"case layer norm infinite weight {C}", flush=True)
+    g = torch.Generator().manual_seed(C)
+    for dtype in (BF, F32):
+        x, dy = rand(g, 7, C, dtype=dtype), rand(g, 7, C, dtype=dtype)
+        w = torch.ones(C)
+        w[-1] = float("inf")
+        _, mean, rstd = ops.layer_norm_forward(x.to(DEV), w.to(DEV), stats=True)
+        dx = ops.layer_norm_backward(dy.to(DEV), x.to(DEV), mean, rstd, w.to(DEV))[0].cpu().double()
+        xd = x.double()
+        xh = (xd - xd.mean(-1, keepdim=True)) / (xd.var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+        a = dy.double() * w.double()
+        want = a - a.mean(-1, keepdim=True) - xh * (a * xh).mean(-1, keepdim=True)
+        assert torch.equal(torch.isnan(dx), torch.isnan(want)) and torch.equal(torch.isinf(dx), torch.isinf(want))
+        assert torch.isinf(want).any()
+
+
 def test_gated_ffn_many_rows():
     """Rows beyond one range of the weight gradients' sums, a ragged end, gradients kept in fp32."""
     print("case gated ffn 2500 rows", flush=True)
