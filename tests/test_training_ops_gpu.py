@@ -706,6 +706,14 @@ def test_parcae_trunk_lm_dropout():
     z0, zin, zlm = (rand(g, 1, n, n, C) for _ in range(3))
     pm = torch.ones(1, n, n, dtype=torch.bool)
     step = iter(range(10))
+    # weights of two types: each gradient in its own, rounded once
+    x = rand(g, 9, 64, dtype=BF).to(DEV)
+    wi, wo = rand(g, 64, 64, scale=0.1).to(DEV).double().requires_grad_(), rand(g, 64, 32, dtype=BF, scale=0.1).to(DEV).requires_grad_()
+    with torch.enable_grad():
+        y = functional.gated_ffn(x, wi, wo)
+        gi, go = torch.autograd.grad(y, [wi, wo], torch.ones_like(y))
+    _, ri, ro = ops.gated_ffn_backward(torch.ones_like(x), x, wi.detach().to(BF), wo.detach(), dw_dtype=F32)
+    assert gi.dtype == torch.float64 and torch.equal(gi, ri.double()) and go.dtype == BF and torch.equal(go, ro.to(BF))
 
     def dropped():
         return ops.dropout_forward(zlm.to(DEV), 0.25, 99, next(step))
