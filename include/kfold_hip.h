@@ -397,13 +397,15 @@ int kfh_layer_norm_backward(const void* dy, const void* x, const float* mean, co
  *   [u; v] = x w_in^T,  y = (silu(u) * v) w_out^T;  x, y: [rows, C], w_in: [2F, C], w_out: [C, F],
  * all row-major of io_dtype, C and F multiples of 8, pointers 16-byte aligned.  KFH_BF16: bf16
  * matrix products with fp32 accumulation, hidden values rounded to bf16 between the products;
- * KFH_F32: products carried to fp32 accuracy (as KFH_ARITH_F32), hidden values kept in fp32. */
+ * KFH_F32: products carried to fp32 accuracy (as KFH_ARITH_F32), hidden values kept in fp32.  `y` must
+ * not be `x`. */
 size_t kfh_gated_ffn_workspace_bytes(long long rows, int C, int F, int backward, int io_dtype);
 int kfh_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, void* y, void* workspace,
                           size_t workspace_bytes, long long rows, int C, int F, int io_dtype, void* stream);
 
 /* Gradients for dy [rows, C]: dx [rows, C] (io_dtype), dw_in [2F, C] and dw_out [C, F] (dw_dtype);
- * each may be NULL.  u and v are computed again from x.  rows = 0 gives zero weight gradients. */
+ * each may be NULL.  u and v are computed again from x.  rows = 0 gives zero weight gradients.
+ * `dx` must be neither `x` nor `dy`. */
 int kfh_gated_ffn_backward(const void* dy, const void* x, const void* w_in, const void* w_out, void* dx,
                            void* dw_in, void* dw_out, int dw_dtype, void* workspace, size_t workspace_bytes,
                            long long rows, int C, int F, int io_dtype, void* stream);

@@ -76,6 +76,7 @@ int kfh_gated_ffn_forward(const void* x, const void* w_in, const void* w_out, vo
     if (!x || !w_in || !w_out || !y) return fail(KFH_EINVAL, "gated_ffn_forward: null pointer argument");
     if (misaligned(x) || misaligned(w_in) || misaligned(w_out) || misaligned(y))
         return fail(KFH_EINVAL, "gated_ffn_forward: tensors must be aligned to 16 bytes");
+    if (y == x) return fail(KFH_EINVAL, "gated_ffn_forward: y must not alias x");
     const size_t need = kfh_gated_ffn_workspace_bytes(rows, C, F, 0, io_dtype);
     if (need && (!workspace || workspace_bytes < need || misaligned(workspace, 256)))
         return fail(KFH_EINVAL, "gated_ffn_forward: workspace %zu bytes, need %zu aligned to 256",

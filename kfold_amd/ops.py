@@ -699,8 +699,8 @@ def gated_ffn_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, 
                       workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``(silu(u) * v) w_out^T`` with ``u, v = chunk(x w_in^T, 2)`` over the last dim of x; w_in [2F, C],
     w_out [C, F], C and F multiples of 8, one dtype: bf16, or fp32 with products of fp32 accuracy.
-    ``workspace`` as in ``trimul_forward`` (``workspace_bytes("gated_ffn", rows=, C=, F=, backward=,
-    dtype=)``)."""
+    ``out`` is not x itself; ``workspace`` as in ``trimul_forward`` (``workspace_bytes("gated_ffn",
+    rows=, C=, F=, backward=, dtype=)``)."""
     dev = _require_cuda(x, w_in, w_out, out)
     io = _io_dtype(x)
     rows, C, F = _ffn_shapes(x, w_in, w_out)
@@ -723,7 +723,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_
                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """``(dx, dw_in, dw_out)`` of ``gated_ffn_forward`` for the gradient dy of its result (the hidden
     values are computed again from x); the weight gradients in ``dw_dtype`` (default: the weights'),
-    None for what is not needed.  ``out`` is for dx (not dy itself)."""
+    None for what is not needed.  ``out`` is for dx (neither x nor dy itself)."""
     dev = _require_cuda(dy, x, w_in, w_out, out)
     io = _io_dtype(x)
     rows, C, F = _ffn_shapes(x, w_in, w_out)

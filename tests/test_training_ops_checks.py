@@ -64,6 +64,7 @@ def test_gated_ffn_checks(env):
     _expect(lib, f(p[0], p[1], p[2], p[3], p[4], 1 << 20, 10, 64, 64, 3, None), EINVAL, "io_dtype 3")
     _expect(lib, f(p[0], None, p[2], p[3], p[4], 1 << 20, 10, 64, 64, 0, None), EINVAL, "null")
     _expect(lib, f(p[0] + 2, p[1], p[2], p[3], p[4], 1 << 20, 10, 64, 64, 0, None), EINVAL, "16 bytes")
+    _expect(lib, f(p[0], p[1], p[2], p[0], p[4], 1 << 20, 10, 64, 64, 0, None), EINVAL, "alias")
     need = ws(10, 72, 64, 0, 1)
     _expect(lib, f(p[0], p[1], p[2], p[3], p[4], need - 1, 10, 72, 64, 1, None), EINVAL, "workspace", str(need))
     _expect(lib, f(p[0], p[1], p[2], p[3], None, need, 10, 72, 64, 1, None), EINVAL, "workspace")
