@@ -271,7 +271,7 @@ def test_gated_ffn_forward_and_backward(M, C, F, dtype):
 
 
 @pytest.mark.parametrize("M,C,F", [(33001, 24, 40), (32900, 8, 136), (16400, 64, 32), (16385, 64, 96), (16500, 128, 64),
-                                   (16384, 256, 160)])
+                                   (16500, 128, 96), (16384, 256, 160), (16400, 256, 32)])
 def test_gated_ffn_big_tiles(M, C, F):
     """Enough rows for every kernel to take its large tiles, or for the kernels that keep the rows in
     registers (C = 64, 128, 256), with ragged edges on all sides."""
@@ -303,6 +303,32 @@ def test_layer_norm_infinite_weight(C):
         want = a - a.mean(-1, keepdim=True) - xh * (a * xh).mean(-1, keepdim=True)
         assert torch.equal(torch.isnan(dx), torch.isnan(want)) and torch.equal(torch.isinf(dx), torch.isinf(want))
         assert torch.isinf(want).any()
+
+
+@pytest.mark.parametrize("M,C,F", [(33_000, 136, 264), (33_000, 264, 264), (20_000, 264, 136), (70_000, 256, 288)])
+def test_gated_ffn_largest_tiles(M, C, F):
+    """The 256 x 256, 256 x 128 and 128 x 128 tiles on row-major hidden values and on blocks of them."""
+    print(f"case gated ffn largest tiles {M} x {C} x {F}", flush=True)
+    test_gated_ffn_big_tiles(M, C, F)
+
+
+def test_gated_ffn_bad_rows_among_many():
+    """As test_gated_ffn_saturated_and_bad_rows, for the kernels that keep the rows in registers."""
+    print("case gated ffn bad rows among many", flush=True)
+    for C, F in ((64, 32), (128, 32), (256, 32)):
+        M = 16_390
+        x, w_in, w_out, dy = (t.to(DEV) for t in ffn_inputs(M, C, F, BF, 13))
+        y, dx = ops.gated_ffn_forward(x, w_in, w_out), ops.gated_ffn_backward(dy, x, w_in, w_out)[0]
+        bad = x.clone()
+        rows = (7, 4099, M - 1)
+        for r in rows:
+            bad[r, r % C] = float("nan")
+        yb = ops.gated_ffn_forward(bad, w_in, w_out)
+        dxb = ops.gated_ffn_backward(dy, bad, w_in, w_out)[0]
+        for r in rows:
+            assert torch.isnan(yb[r]).all() and torch.isnan(dxb[r]).all()
+            yb[r], dxb[r] = y[r], dx[r]
+        assert torch.equal(yb, y) and torch.equal(dxb, dx)
 
 
 def test_gated_ffn_many_rows():
@@ -680,6 +706,14 @@ def test_modules_and_mixed_types():
         y = drop(ar, rr, seed=8)
         ga, gr = torch.autograd.grad(y, [ar, rr], torch.ones_like(y))
     assert torch.equal(gr, torch.ones_like(gr)) and torch.equal(ga, ops.dropout_backward(torch.ones_like(a), 0.3, 8, 0, 2))
+    # weights of two types: each gradient in its own, rounded once
+    x = rand(g, 9, 64, dtype=BF).to(DEV)
+    wi, wo = rand(g, 64, 64, scale=0.1).to(DEV).double().requires_grad_(), rand(g, 64, 32, dtype=BF, scale=0.1).to(DEV).requires_grad_()
+    with torch.enable_grad():
+        y = functional.gated_ffn(x, wi, wo)
+        gi, go = torch.autograd.grad(y, [wi, wo], torch.ones_like(y))
+    _, ri, ro = ops.gated_ffn_backward(torch.ones_like(x), x, wi.detach().to(BF), wo.detach(), dw_dtype=F32)
+    assert gi.dtype == torch.float64 and torch.equal(gi, ri.double()) and go.dtype == BF and torch.equal(go, ro.to(BF))
     # a device seed changed in place before the backward pass is an error, not another mask
     s = torch.tensor([8]).to(DEV)
     with torch.enable_grad():
@@ -706,14 +740,6 @@ def test_parcae_trunk_lm_dropout():
     z0, zin, zlm = (rand(g, 1, n, n, C) for _ in range(3))
     pm = torch.ones(1, n, n, dtype=torch.bool)
     step = iter(range(10))
-    # weights of two types: each gradient in its own, rounded once
-    x = rand(g, 9, 64, dtype=BF).to(DEV)
-    wi, wo = rand(g, 64, 64, scale=0.1).to(DEV).double().requires_grad_(), rand(g, 64, 32, dtype=BF, scale=0.1).to(DEV).requires_grad_()
-    with torch.enable_grad():
-        y = functional.gated_ffn(x, wi, wo)
-        gi, go = torch.autograd.grad(y, [wi, wo], torch.ones_like(y))
-    _, ri, ro = ops.gated_ffn_backward(torch.ones_like(x), x, wi.detach().to(BF), wo.detach(), dw_dtype=F32)
-    assert gi.dtype == torch.float64 and torch.equal(gi, ri.double()) and go.dtype == BF and torch.equal(go, ro.to(BF))
 
     def dropped():
         return ops.dropout_forward(zlm.to(DEV), 0.25, 99, next(step))
