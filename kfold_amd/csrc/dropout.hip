@@ -10,6 +10,9 @@
 // and the scale uses the same multiple, so the expectation of y is exact.  The gradient is the same
 // map applied to dy.  Dropped values are never multiplied: inf and NaN there leave 0.
 // The product and the sum are fp32, rounded once.
+//
+// Bound by memory traffic, the generator (about 60 VALU instructions per call) beside it: 768 x 768 x 128 bf16
+// row-wise with residual 86 us (453 MB, 5.3 TB/s), 32.9 M fp32 with a mask value each 48.5 us (263 MB, 5.4 TB/s).
 #include "train.hpp"
 
 namespace kfh {

