@@ -11,7 +11,7 @@ from tests.test_hostsim_address_walk import _untouched
 from tests.test_hostsim_parity import _twin
 
 # streams and graphs of a device; minutes of CPU time
-SKIP = {"test_training_ops_streams_and_graphs", "test_gated_ffn_largest_tiles"}
+SKIP = {"test_training_ops_streams_and_graphs", "test_training_ops_two_graphs", "test_gated_ffn_largest_tiles"}
 
 for _attr, _fn in list(vars(_mod).items()):
     if _attr.startswith("test_") and callable(_fn) and _attr not in SKIP:

@@ -679,6 +679,45 @@ def test_transition_training_step(dtype):
     assert err <= 8 * 2.0 ** -9, err
 
 
+def test_transition_training_under_autocast():
+    """fp32 tensors under bf16 autocast: bf16 products on the rounded normalised rows, fp32 results and
+    gradients; a forward pass inside and the backward pass outside of it."""
+    print("case transition under autocast", flush=True)
+    C = 64
+    mod = layers.Transition(C, 2)
+    synthetic.init_weights_(mod, 3, std=0.1)
+    mod = mod.to(DEV)
+    g = torch.Generator().manual_seed(14)
+    x, dy = rand(g, 2, 9, C).to(DEV).requires_grad_(), rand(g, 2, 9, C).to(DEV)
+    params = list(mod.parameters())
+    with torch.enable_grad():
+        with torch.autocast(x.device.type, dtype=BF):
+            y = mod(x)
+        grads = torch.autograd.grad(y, [x] + params, dy)
+        xn = functional.layer_norm(x, mod.layernorm.weight, mod.layernorm.bias, mod.layernorm.eps)
+        want = functional.gated_ffn(xn.to(BF), mod.swiglu.linear.weight, mod.linear_out.weight).float()
+        wg = torch.autograd.grad(want, [x] + params, dy)
+    assert y.dtype == F32 and torch.equal(y, want)
+    assert all(p.dtype == F32 and torch.equal(p, q) for p, q in zip(grads, wg))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_functional_gradients_of_some_inputs(dtype):
+    """Frozen inputs change nothing in the gradients of the others."""
+    print(f"case gradients of some inputs {dtype}", flush=True)
+    g = torch.Generator().manual_seed(15)
+    x, w_in, w_out, dy = (t.to(DEV) for t in ffn_inputs(45, 64, 32, dtype, 15))
+    lw, lb = (1 + rand(g, 64, scale=0.2)).to(DEV), rand(g, 64, scale=0.1).to(DEV)
+    for f, args in ((functional.gated_ffn, (x, w_in, w_out)), (functional.layer_norm, (x, lw, lb))):
+        def run(which):
+            leaves = [t.clone().requires_grad_(k in which) for k, t in enumerate(args)]
+            with torch.enable_grad():
+                return torch.autograd.grad(f(*leaves), [leaves[k] for k in which], dy)
+        full = run((0, 1, 2))
+        for which in ((0,), (1,), (2,), (0, 2), (1, 2)):
+            assert all(torch.equal(p, full[k]) for p, k in zip(run(which), which)), (f, which)
+
+
 def test_modules_and_mixed_types():
     print("case modules", flush=True)
     g = torch.Generator().manual_seed(6)
@@ -802,3 +841,40 @@ def test_training_ops_streams_and_graphs():
     assert torch.equal(y.detach(), want[0])
     assert torch.equal(grads[3], want[2]) and torch.equal(grads[4], want[3]) and torch.equal(grads[1], want[4])
     assert torch.equal(grads[0], dy + want[1])
+
+
+@pytest.mark.parametrize("M,C,F,dtype", [(16_390, 128, 64, BF), (16_390, 256, 64, BF), (12, 64, 32, BF), (3000, 136, 264, BF),
+                                         (70, 128, 256, F32)])
+def test_training_ops_two_graphs(M, C, F, dtype):
+    """Two recorded steps of different inputs that live side by side, replayed in turn and on two streams
+    at once with eager work between: same bits as eager calls."""
+    print(f"case two graphs {M} x {C} x {F} {dtype}", flush=True)
+    sets = [[t.to(DEV) for t in ffn_inputs(M, C, F, dtype, 40 + k)] for k in range(2)]
+
+    def step(x, w_in, w_out, dy):
+        xn, mean, rstd = ops.layer_norm_forward(x, stats=True)
+        y = ops.gated_ffn_forward(xn, w_in, w_out)
+        dxn, dwi, dwo = ops.gated_ffn_backward(dy, xn, w_in, w_out)
+        return (y, dwi, dwo) + ops.layer_norm_backward(dxn, x, mean, rstd)
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph() for _ in sets], []
+    for graph, s in zip(graphs, sets):
+        with torch.cuda.graph(graph):
+            held.append(step(*s))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for k in range(4):
+        for t in (t for h in held for t in h):
+            t.zero_()
+        torch.cuda.synchronize()
+        for i, graph in enumerate(graphs):
+            if k % 2:
+                with torch.cuda.stream(streams[i]):
+                    graph.replay()
+            else:
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for h, w in zip(held, want) for p, q in zip(h, w)), k
+        assert all(torch.equal(p, q) for p, q in zip(step(*sets[k % 2]), want[k % 2])), k
+        torch.cuda.synchronize()
