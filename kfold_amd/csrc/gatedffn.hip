@@ -207,7 +207,7 @@ template <int P, int TM, int TN, int OUT> struct GemmLds {
 };
 
 template <int P, int AK, int BK_, int OUT, int TM, int TN>
-__global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
+__device__ __forceinline__ void gemm_tile(
     const void* __restrict__ A, long long lda, long long ap, const void* __restrict__ B, long long ldb, long long bp,
     void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits, const void* __restrict__ A2,
     long long lda2, long long ap2, const void* __restrict__ B2, int Mo2) {
@@ -313,6 +313,21 @@ __global__ __launch_bounds__((Waves<TM, TN>::NW * 64)) void ffn_gemm_kernel(
         __syncthreads();
         Out::flush(smem, base, No, m0, Mo, n0 + c * RN, No, tid);
     }
+}
+// a name per workgroup size
+template <int P, int AK, int BK_, int OUT, int TM, int TN>
+__global__ __launch_bounds__(256) void ffn_gemm_kernel(
+    const void* __restrict__ A, long long lda, long long ap, const void* __restrict__ B, long long ldb, long long bp,
+    void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits, const void* __restrict__ A2,
+    long long lda2, long long ap2, const void* __restrict__ B2, int Mo2) {
+    gemm_tile<P, AK, BK_, OUT, TM, TN>(A, lda, ap, B, ldb, bp, out, Mo, No, K, kper, splits, A2, lda2, ap2, B2, Mo2);
+}
+template <int P, int AK, int BK_, int OUT, int TM, int TN>
+__global__ __launch_bounds__(512) void ffn_gemm_large_kernel(
+    const void* __restrict__ A, long long lda, long long ap, const void* __restrict__ B, long long ldb, long long bp,
+    void* __restrict__ out, long long Mo, int No, long long K, long long kper, int splits, const void* __restrict__ A2,
+    long long lda2, long long ap2, const void* __restrict__ B2, int Mo2) {
+    gemm_tile<P, AK, BK_, OUT, TM, TN>(A, lda, ap, B, ldb, bp, out, Mo, No, K, kper, splits, A2, lda2, ap2, B2, Mo2);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -549,9 +564,13 @@ template <int P, int AK, int BK_, int OUT, int TM, int TN>
 static void gemm(Operand a, Operand b, void* out, long long Mo, int No, long long K, long long kper, int splits,
                  hipStream_t stream, Operand a2 = {}, Operand b2 = {}, int Mo2 = 0) {
     const long long mt = up_div(Mo, TM) + up_div(Mo2, TM), nt = up_div(No, TN);
-    hipLaunchKernelGGL((ffn_gemm_kernel<P, AK, BK_, OUT, TM, TN>),
-                       dim3(OUT == OUT_PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt)), dim3(Waves<TM, TN>::NW * 64), 0,
-                       stream, a.p, a.ld, a.plane, b.p, b.ld, b.plane, out, Mo, No, K, kper, splits, a2.p, a2.ld, a2.plane, b2.p, Mo2);
+    const dim3 grid(OUT == OUT_PART ? xcd_grid(splits, (int)(mt * nt)) : xcd_grid(mt, (int)nt));
+    if constexpr (Waves<TM, TN>::NW == 8)
+        hipLaunchKernelGGL((ffn_gemm_large_kernel<P, AK, BK_, OUT, TM, TN>), grid, dim3(512), 0, stream, a.p, a.ld, a.plane, b.p, b.ld,
+                           b.plane, out, Mo, No, K, kper, splits, a2.p, a2.ld, a2.plane, b2.p, Mo2);
+    else
+        hipLaunchKernelGGL((ffn_gemm_kernel<P, AK, BK_, OUT, TM, TN>), grid, dim3(256), 0, stream, a.p, a.ld, a.plane, b.p, b.ld, b.plane,
+                           out, Mo, No, K, kper, splits, a2.p, a2.ld, a2.plane, b2.p, Mo2);
 }
 
 // out [Mo, No] = A [Mo, K] (AK) times B, [No, K] (K_MAJOR) or [K, No] (R_MAJOR); part: product_part_bytes.

@@ -65,12 +65,10 @@ __device__ __forceinline__ void store_hidden(uint16_t* t, size_t slot, bool live
     __builtin_nontemporal_store(live ? __builtin_bit_cast(u32x4, f1) : none, o + 64);
 }
 
-template <int KS, bool BWD, bool FUSE, int NW, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t* __restrict__ x,
-                                                                  const uint16_t* __restrict__ dy,
-                                                                  const u32x4* __restrict__ wp, uint16_t* __restrict__ h,
-                                                                  uint16_t* __restrict__ d, uint16_t* __restrict__ out, long long M,
-                                                                  int F) {
+template <int KS, bool BWD, bool FUSE, int NW>
+__device__ __forceinline__ void stream_rows(const uint16_t* __restrict__ x, const uint16_t* __restrict__ dy,
+                                            const u32x4* __restrict__ wp, uint16_t* __restrict__ h, uint16_t* __restrict__ d,
+                                            uint16_t* __restrict__ out, long long M, int F) {
     constexpr int C = 16 * KS, NF = stream_frags<KS, BWD, FUSE>(), NT = NW * 64, NB = FUSE ? KS / 2 : 1;
     // backward: the weights of the next step come in two halves, one during the first products and one during
     // the activation and the second products, with half the registers on the way (147456 x 128 x 256: 179 ->
@@ -206,19 +204,43 @@ __global__ __launch_bounds__(NW * 64, OCC) void ffn_stream_kernel(const uint16_t
     }
 }
 
+// a name per workgroup size: up to C = 128 workgroups of 4 wavefronts (backward two, forward three on a CU), at
+// C = 256 one of 8
+template <int KS, bool BWD>
+__global__ __launch_bounds__(256, (BWD ? 2 : 3)) void ffn_stream_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ dy,
+                                                                        const u32x4* __restrict__ wp, uint16_t* __restrict__ h,
+                                                                        uint16_t* __restrict__ d, uint16_t* __restrict__ out,
+                                                                        long long M, int F) {
+    stream_rows<KS, BWD, true, 4>(x, dy, wp, h, d, out, M, F);
+}
+template <int KS, bool BWD>
+__global__ __launch_bounds__(512, 2) void ffn_stream_wide_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ dy,
+                                                                 const u32x4* __restrict__ wp, uint16_t* __restrict__ h,
+                                                                 uint16_t* __restrict__ d, uint16_t* __restrict__ out,
+                                                                 long long M, int F) {
+    stream_rows<KS, BWD, false, 8>(x, dy, wp, h, d, out, M, F);
+}
+
 template <int KS, bool BWD>
 static void stream_t(const void* x, const void* dy, const void* w_in, const void* w_out, void* pack, void* h, void* d,
                      void* out, long long M, int F, hipStream_t stream) {
     constexpr bool FUSE = KS <= 8;
-    constexpr int NW = KS == 16 ? 8 : 4, OCC = BWD || KS == 16 ? 2 : 3;
+    constexpr int NW = FUSE ? 4 : 8;
     const long long slots = (long long)(F / 32) * stream_frags<KS, BWD, FUSE>() * 64;
     hipLaunchKernelGGL((ffn_pack_kernel<KS, BWD, FUSE>), dim3((unsigned)((slots + 255) / 256)), dim3(256), 0, stream,
                        static_cast<const uint16_t*>(w_in), static_cast<const uint16_t*>(w_out), static_cast<u32x4*>(pack), F,
                        slots);
-    hipLaunchKernelGGL((ffn_stream_kernel<KS, BWD, FUSE, NW, OCC>), dim3((unsigned)((M + 32 * NW - 1) / (32 * NW))), dim3(NW * 64),
-                       0, stream, static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(dy),
-                       static_cast<const u32x4*>(pack), static_cast<uint16_t*>(h), static_cast<uint16_t*>(d),
-                       static_cast<uint16_t*>(out), M, F);
+    const dim3 grid((unsigned)((M + 32 * NW - 1) / (32 * NW))), block(NW * 64);
+    const uint16_t* const xs = static_cast<const uint16_t*>(x);
+    const uint16_t* const dys = static_cast<const uint16_t*>(dy);
+    const u32x4* const wp = static_cast<const u32x4*>(pack);
+    uint16_t* const hs = static_cast<uint16_t*>(h);
+    uint16_t* const ds = static_cast<uint16_t*>(d);
+    uint16_t* const outs = static_cast<uint16_t*>(out);
+    if constexpr (FUSE)
+        hipLaunchKernelGGL((ffn_stream_kernel<KS, BWD>), grid, block, 0, stream, xs, dys, wp, hs, ds, outs, M, F);
+    else
+        hipLaunchKernelGGL((ffn_stream_wide_kernel<KS, BWD>), grid, block, 0, stream, xs, dys, wp, hs, ds, outs, M, F);
 }
 
 size_t ffn_stream_pack_bytes(int C, int F, int backward) {
