@@ -39,7 +39,7 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src.name}:\n{err}")
+        raise RuntimeError(f"hipcc failed for {src.name}, exit status {res.returncode}:\n{err}")
     if err.strip() and verbose:
         print(err, file=sys.stderr)
 
@@ -59,7 +59,7 @@ def _asm_of(src: Path) -> str:
     res = subprocess.run([HIPCC, *FLAGS, "--cuda-device-only", "-S", str(src), "-o", "-"],
                          capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc -S failed for {src.name}:\n{res.stderr[-2000:]}")
+        raise RuntimeError(f"hipcc -S failed for {src.name}, exit status {res.returncode}:\n{res.stderr[-2000:]}")
     return res.stdout
 
 
@@ -123,6 +123,9 @@ def kernel_facts(jobs: int = 8, srcs: list[Path] | None = None) -> tuple[dict[st
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
+    """Compile and link the library, then write the records of its kernels.  The library is put in its
+    place when it is whole, so that a build that fails leaves the one of the last good build; records
+    that cannot be made are left out (their readers look for the files), and the reason is printed."""
     objdir = CSRC / "_obj"
     objdir.mkdir(exist_ok=True)
     srcs = sources()
@@ -130,15 +133,23 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     jobs = jobs or min(len(srcs), os.cpu_count() or 4, 16)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         list(ex.map(lambda so: _compile(so[0], so[1], verbose), zip(srcs, objs)))
-    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(LIB), *map(str, objs)]
+    linked = objdir / LIB.name
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(linked), *map(str, objs)]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"link failed:\n{res.stderr}")
+        raise RuntimeError(f"link failed, exit status {res.returncode}:\n{res.stderr}")
+    os.replace(linked, LIB)
     import json
 
-    isa, resources = kernel_facts(jobs)
+    for record in (ISA_JSON, RESOURCES_JSON):
+        record.unlink(missing_ok=True)
+    try:
+        isa, resources = kernel_facts(jobs)
+    except (OSError, RuntimeError) as e:
+        print(f"the library is built, the records of its kernels are not: {e}", file=sys.stderr, flush=True)
+        return LIB
     ISA_JSON.write_text(json.dumps(isa, indent=1) + "\n")
     RESOURCES_JSON.write_text(json.dumps(resources, indent=1) + "\n")
     return LIB
