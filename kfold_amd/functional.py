@@ -2,16 +2,28 @@
 
 Each is one ``torch.autograd.Function`` around the forward and backward entry points; what is kept
 between the two is the operator's inputs (for the layer norm also two fp32 statistics per row).  First
-derivatives only.  To record a step into a HIP graph, call the forward and backward functions of
+derivatives in reverse mode only: forward-mode tangents are refused.  To record a step into a HIP graph, call the forward and backward functions of
 ``ops`` themselves: they only enqueue kernels on the current stream.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
+
+
+def _differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether the call has to go through the autograd function: gradients are wanted, or an argument
+    carries a tangent, which the function refuses (the kernels would drop it)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    # tangents exist inside a dual level only; asking each tensor costs microseconds
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -34,7 +46,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dim of x (bf16 or fp32, any width), result in x.dtype."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     return ops.layer_norm_forward(x, weight, bias, eps)
 
@@ -60,7 +72,7 @@ class _GatedFFN(torch.autograd.Function):
 def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> torch.Tensor:
     """``(silu(u) * v) w_out^T`` with ``u, v = chunk(x w_in^T, 2)``: the SwiGLU block with its output
     projection.  Weights of another dtype are rounded to x's first; their gradients come in their own."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_in, w_out)):
+    if _differentiated(x, w_in, w_out):
         return _GatedFFN.apply(x, w_in, w_out)
     return ops.gated_ffn_forward(x, w_in.to(x.dtype), w_out.to(x.dtype))
 
@@ -88,6 +100,6 @@ class _Dropout(torch.autograd.Function):
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, shared_dim: int | None = None,
             residual: torch.Tensor | None = None) -> torch.Tensor:
     """``(residual or 0) + dropout(x)`` with the mask of ``ops.dropout_forward``."""
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _differentiated(x, residual):
         return _Dropout.apply(x, residual, p, seed, offset, shared_dim)
     return ops.dropout_forward(x, p, seed, offset, shared_dim, residual)
