@@ -30,5 +30,5 @@ class Dropout(nn.Module):
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x
         if seed is None:
-            seed = int(torch.randint(0, 2 ** 62, ()))
+            seed = int(torch.randint(0, 2 ** 62, (), device="cpu"))       # whatever torch's default device is
         return functional.dropout(x, self.p, seed, offset, self.shared_dim, residual)

@@ -35,3 +35,17 @@ def test_forward_mode_tangents_are_refused(grad):
         # without a tangent the same calls run; dropout that does nothing keeps the tangent
         assert functional.layer_norm(x, w, w).shape == functional.gated_ffn(x, w_in, w_out).shape == x.shape
         assert torch.equal(fwad.unpack_dual(primitives.Dropout(0.3).eval()(dx)).tangent, t)
+
+
+def test_dropout_seed_comes_from_the_cpu_generator():
+    """Under another default device too: there a drawn seed would belong to that device's generator, and
+    reading it would wait for the device."""
+    x = _rand(40, 64)
+    drop = primitives.Dropout(0.3)
+    with hostsim.host_backend():
+        torch.manual_seed(1)
+        want = drop(x)
+        torch.manual_seed(1)
+        with torch.device("meta"):
+            got = drop(x)
+    assert torch.equal(got, want)
