@@ -65,7 +65,7 @@ class _GatedFFN(torch.autograd.Function):
         # one rounding to the weights' type: in the kernel where both have the type it writes
         same = w_in.dtype == w_out.dtype == torch.bfloat16
         dx, dwi, dwo = ops.gated_ffn_backward(dy, x, w_in.to(x.dtype), w_out.to(x.dtype), need_dx=need_x,
-                                              need_dw=need_i or need_o, dw_dtype=torch.bfloat16 if same else torch.float32)
+                                              need_dw=(need_i, need_o), dw_dtype=torch.bfloat16 if same else torch.float32)
         return dx, dwi.to(w_in.dtype) if need_i else None, dwo.to(w_out.dtype) if need_o else None
 
 

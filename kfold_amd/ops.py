@@ -719,11 +719,13 @@ def gated_ffn_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, 
 
 
 def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
-                       need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype | None = None,
+                       need_dx: bool = True, need_dw: bool | tuple[bool, bool] = True,
+                       dw_dtype: torch.dtype | None = None,
                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """``(dx, dw_in, dw_out)`` of ``gated_ffn_forward`` for the gradient dy of its result (the hidden
     values are computed again from x); the weight gradients in ``dw_dtype`` (default: the weights'),
-    None for what is not needed.  ``out`` is for dx (neither x nor dy itself)."""
+    None for what is not needed; ``need_dw`` may be a pair, for dw_in and dw_out.  ``out`` is for dx
+    (neither x nor dy itself)."""
     dev = _require_cuda(dy, x, w_in, w_out, out)
     io = _io_dtype(x)
     rows, C, F = _ffn_shapes(x, w_in, w_out)
@@ -734,11 +736,10 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_
         raise TypeError(f"hip backend supports bfloat16 and float32 tensors, got dw_dtype={dw_dtype}")
     xc, dyc, wi, wo = _aligned(x), _aligned(dy), _aligned(w_in), _aligned(w_out)
     dx = _result(out, xc, "out", aligned=True) if need_dx else None
-    dwi = dwo = None
-    if need_dw:
-        dwi = torch.empty(tuple(w_in.shape), dtype=dw_dtype, device=dev)
-        dwo = torch.empty(tuple(w_out.shape), dtype=dw_dtype, device=dev)
-    if not (need_dx or need_dw):
+    need_i, need_o = need_dw if isinstance(need_dw, (tuple, list)) else (need_dw, need_dw)
+    dwi = torch.empty(tuple(w_in.shape), dtype=dw_dtype, device=dev) if need_i else None
+    dwo = torch.empty(tuple(w_out.shape), dtype=dw_dtype, device=dev) if need_o else None
+    if not (need_dx or need_i or need_o):
         return None, None, None
     L = _lib.lib()
     ws_bytes = L.kfh_gated_ffn_workspace_bytes(rows, C, F, 1, io)

@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
-from kfold_amd import functional, layers, primitives
+from kfold_amd import functional, layers, ops, primitives
 from tests import hostsim
 
 
@@ -49,3 +49,21 @@ def test_dropout_seed_comes_from_the_cpu_generator():
         with torch.device("meta"):
             got = drop(x)
         assert torch.equal(got, want)              # (the host build's memory ends with its context)
+
+
+def test_frozen_weights_are_not_asked_for(monkeypatch):
+    """The backward call computes the gradients that somebody wants, each weight by itself."""
+    asked = []
+
+    def backward(*args, _call=ops.gated_ffn_backward, **kwargs):
+        got = _call(*args, **kwargs)
+        asked.append(tuple(t is not None for t in got))
+        return got
+    monkeypatch.setattr(ops, "gated_ffn_backward", backward)
+    args = (_rand(5, 64), _rand(64, 64, seed=4, scale=0.1), _rand(64, 32, seed=5, scale=0.1))
+    with hostsim.host_backend(), torch.enable_grad():
+        for k in range(1, 8):
+            want = tuple(bool(k >> i & 1) for i in range(3))
+            leaves = [t.clone().requires_grad_(w) for t, w in zip(args, want)]
+            functional.gated_ffn(*leaves).sum().backward()
+            assert asked.pop() == want
