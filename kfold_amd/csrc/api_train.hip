@@ -31,7 +31,7 @@ int kfh_layer_norm_forward(const void* x, const float* weight, const float* bias
 
 size_t kfh_layer_norm_backward_workspace_bytes(long long rows, int C) {
     if (rows < 0 || rows > kMaxRows || C < 1 || C > 65536) return 0;
-    return align_up((size_t)ln_bwd_blocks(rows, C) * 2 * C * sizeof(float));
+    return align_up((size_t)ln_bwd_blocks(rows) * 2 * C * sizeof(float));
 }
 
 int kfh_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd, const float* weight,

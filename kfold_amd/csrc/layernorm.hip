@@ -6,13 +6,17 @@
 //   dx     = rstd * (a - mean_c(a) - xh * mean_c(a * xh))
 //   dgamma = sum_rows dy * xh,   dbeta = sum_rows dy
 //
-// Statistics, row sums and the sums over rows are held in fp32; y and dx are rounded once, when they
-// are stored.  The variance is taken from the deviations (two passes over the row), so a row far
-// from zero loses nothing.  The sums over rows go through per-workgroup partial sums that one more
-// kernel adds in a fixed order: the same call gives the same bits.
+// Statistics, row sums and a workgroup's sums over its rows are held in fp32; y and dx are rounded once, when
+// they are stored.  The variance is taken from the deviations (two passes over the row), so a row far
+// from zero loses no more than its mean's rounding.  The sums over rows go through per-workgroup partial sums that
+// one more kernel adds in 64 bits, in a fixed order: the same call gives the same bits.
 //
-// Bound by memory traffic: every value is read once.  589824 x 256 bf16 forward 102 us (5.9 TB/s; a copy of
-// 1 GiB reaches 5.1), 147456 x 128 bf16 backward with the sums 25.5 us (21 + 4 for the partial sums; 114 MB).
+// Bound by memory traffic.  Up to 2048 channels every value is read once: 589824 x 256 bf16 forward 103 us
+// (5.9 TB/s; a copy of 1 GiB, half of it writes, reaches 5.1), 147456 x 128 bf16 backward with the sums 25 us (21 + 4 for
+// the partial sums; 114 MB).  Wider rows are read three times forward (the sum, the deviations, the result) and
+// three times backward (the column sums, the row sums, dx), mostly from the caches: 16384 x 4096 bf16 1.3 TB/s
+// forward, 1.5 backward (2048 channels: 5.0, 4.2).
+// Widths that are no multiple of 8 go through single elements: 5001 x 765 fp32 backward 17 us (46 MB).
 #include "train.hpp"
 
 namespace kfh {
@@ -144,7 +148,9 @@ __global__ __launch_bounds__(256) void ln_fwd_reg_kernel(const void* x, const fl
     using Row = RegRow<IO, VEC, LPR, NJ>;
     constexpr int N = NJ * 8, RPB = 256 / LPR;              // rows side by side in the workgroup
     const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
-    const float fc = (float)C;               // divided by, not multiplied with 1 / C: a constant row gives exactly 0
+    // divided by, not multiplied with a rounded 1 / C: a row of one value gives exactly 0 where its sum is exact, as
+    // with bf16 values (8 bits, at most 2048 of them)
+    const float fc = (float)C;
     float gam[N], bet[N];
     Row::params(gamma, 1.f, C, l, gam);
     Row::params(beta, 0.f, C, l, bet);
@@ -402,14 +408,13 @@ static bool by_width(int C, F f) {
     return true;
 }
 
-// workgroups of four rows each; beyond 2^20 of them a workgroup takes several
+// workgroups for M rows of which one takes `rows` at a time; beyond 2^20 of them a workgroup takes several turns
 static unsigned row_grid(long long M, long long rows) { return (unsigned)min((M + rows - 1) / rows, 1LL << 20); }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // partial rows of a backward call: enough workgroups to fill the chip with a few each, and enough rows
 // per workgroup (16) that the partial sums stay small beside the rows
-int ln_bwd_blocks(long long M, int C) {
-    (void)C;
+int ln_bwd_blocks(long long M) {
     return (int)max(1LL, min((M + 15) / 16, 1024LL));
 }
 
@@ -444,7 +449,7 @@ static void ln_backward_t(const void* dy, const void* x, const float* mean, cons
                           void* dx, float* dgamma, float* dbeta, float* part, long long M, int C, hipStream_t stream) {
     const dim3 block(256);
     const bool sums = dgamma || dbeta;
-    const int nblk = ln_bwd_blocks(M, C);
+    const int nblk = ln_bwd_blocks(M);
     const bool vec = C % 8 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gamma);
     const bool done = by_width(C, [&](auto lpr, auto nj) {
         constexpr int LPR = decltype(lpr)::v, NJ = decltype(nj)::v, R = NJ == 1 ? 2 : 1;

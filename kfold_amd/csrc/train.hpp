@@ -8,8 +8,8 @@ namespace kfh {
 // gamma, beta: fp32 [C] or null; mean, rstd: fp32 [M], both or neither
 void launch_ln_forward(const void* x, int io_dtype, const float* gamma, const float* beta, void* y, float* mean,
                        float* rstd, long long M, int C, float eps, hipStream_t stream);
-// rows of partial sums a backward call writes: part holds ln_bwd_blocks(M, C) * 2C fp32
-int ln_bwd_blocks(long long M, int C);
+// rows of partial sums a backward call writes: part holds ln_bwd_blocks(M) * 2C fp32
+int ln_bwd_blocks(long long M);
 // dx, dgamma, dbeta may each be null; part may be null if dgamma and dbeta are
 void launch_ln_backward(const void* dy, const void* x, int io_dtype, const float* mean, const float* rstd,
                         const float* gamma, void* dx, float* dgamma, float* dbeta, float* part, long long M, int C,
