@@ -494,8 +494,17 @@ static size_t product_part_bytes(long long Mo, long long No, long long K, int io
     return s > 1 ? (size_t)s * Mo * No * 4 : 0;
 }
 
-// The streamed kernels: bf16, a width they are built for, whole steps of hidden channels, and rows enough
-// to give every CU a workgroup (below that their 128 or 256 rows per workgroup leave CUs idle).
+// The streamed kernels: bf16, a width they are built for, whole steps of hidden channels, and 16384 rows, which
+// give them 128 workgroups of 128 rows (C <= 128) or 64 of 256 rows (C = 256): fewer leave too many of the 256 CUs
+// idle.  Tiles against streamed kernels, us, forward | backward:
+//     C x F          8192 rows                 16384                     32768                     65536
+//     64 x 128       12.3 12.2 | 25.5 24.8     12.2 12.0 | 34.5 29.1     12.1 11.7 | 38.9 35.3     19.1 11.9 | 53.5 46.8
+//     128 x 256      12.3 14.3 | 40.1 40.4     14.8 14.7 | 44.0 43.8     18.6 15.5 | 60.7 53.1     34.8 20.4 | 92.1 76.8
+//     128 x 512      15.3 22.9 | 45.7 56.1     21.2 23.2 | 64.5 63.6     31.1 24.4 | 94.1 81.3     56.6 31.9 | 160 124
+//     256 x 512      19.2 44.8 | 59.9 95.7     26.2 44.6 | 88.3 110      44.7 52.5 | 137 135       80.7 71.2 | 274 201
+//     256 x 1024     28.5 76.0 | 96.9 162      46.1 77.0 | 144 179       79.7 86.9 | 269 228       148 123 | 520 365
+// so the two meet at the threshold for C = 64 and 128, and at 256 only between 32768 and 49152 rows: there the calls
+// from 16384 rows up to that pay up to 1.7 times the tiles' time.
 static bool streamed(long long M, int C, int F, int io_dtype) {
     return io_dtype == KFH_BF16 && (C == 64 || C == 128 || C == 256) && F % 32 == 0 && M >= 16384;
 }
