@@ -12,7 +12,9 @@
 // The product and the sum are fp32, rounded once.
 //
 // Bound by memory traffic, the generator (about 60 VALU instructions per call) beside it: 768 x 768 x 128 bf16
-// row-wise with residual 86 us (453 MB, 5.3 TB/s), 32.9 M fp32 with a mask value each 48.5 us (263 MB, 5.4 TB/s).
+// row-wise with residual 86 us (453 MB, 5.3 TB/s), 32.9 M fp32 with a mask value each 48.5 us (263 MB, 5.4 TB/s) where
+// inputs and outputs change from call to call (a copy of them takes 50), 40 us on the same tensors again and again,
+// which the 256 MB last-level cache then holds in part.
 #include "train.hpp"
 
 namespace kfh {
