@@ -14,7 +14,7 @@
 // Bound by memory traffic.  Up to 2048 channels every value is read once: 589824 x 256 bf16 forward 103 us
 // (5.9 TB/s; a copy of 1 GiB, half of it writes, reaches 5.1), 147456 x 128 bf16 backward with the sums 25 us (21 + 4 for
 // the partial sums; 114 MB).  Wider rows are read three times forward (the sum, the deviations, the result) and
-// three times backward (the column sums, the row sums, dx), mostly from the caches: 16384 x 4096 bf16 1.3 TB/s
+// three times backward (the column sums, the row sums, dx): 16384 x 4096 bf16 1.3 TB/s
 // forward, 1.5 backward (2048 channels: 5.0, 4.2).
 // Widths that are no multiple of 8 go through single elements: 5001 x 765 fp32 backward 17 us (46 MB).
 #include "train.hpp"
